@@ -1,0 +1,763 @@
+// Distillation from a teacher's top logits: the teacher's half (the k largest logits of a row with the row's logsumexp)
+// and the student's half (loss and gradient in one pass over the student's logits).
+//
+// Both work on one row per workgroup.  The row is held in registers, VPT 16-byte vectors per thread, so the logits are
+// read from memory once: at the rates of this part (a few FLOP per byte) the kernels are bound by that read and by the
+// store of the gradient.  Rows wider than the registers of a workgroup are read a second time (VPT = 0).  All arithmetic
+// is fp32; the only rounding to fewer bits is the store of the gradient in the logits' own type.
+#include "common.h"
+
+#define DS_BF16 0
+#define DS_FP16 1
+#define DS_FP32 2
+#define DS_MAX_K 512
+#define DS_MAX_CLASSES 262144      // one bit per class in LDS: 32 KB
+
+typedef _Float16 f16;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+// Rows of an odd width start at any multiple of the element size: global memory takes unaligned 16-byte accesses (the
+// compiler needs to be told that the address has no more than the element's alignment, nothing else changes).
+typedef u32x4 __attribute__((aligned(2))) u32x4_a2;
+
+#define DS_LOG2E 1.44269504088896340736f
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T> struct Pack;
+template <> struct Pack<bf16> {
+    static constexpr int E = 8;
+    static constexpr unsigned FILL = 0xff80ff80u;                  // -inf, -inf
+    static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(r[i] << 16);
+            f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            bf16x2 p = __builtin_convertvector((f32x2){f[2 * i], f[2 * i + 1]}, bf16x2);
+            r[i] = __builtin_bit_cast(unsigned, p);
+        }
+        return r;
+    }
+};
+template <> struct Pack<f16> {
+    static constexpr int E = 8;
+    static constexpr unsigned FILL = 0xfc00fc00u;
+    static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f16x2 p = __builtin_bit_cast(f16x2, (unsigned)r[i]);
+            f[2 * i] = (float)p[0];
+            f[2 * i + 1] = (float)p[1];
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f16x2 p = __builtin_convertvector((f32x2){f[2 * i], f[2 * i + 1]}, f16x2);
+            r[i] = __builtin_bit_cast(unsigned, p);
+        }
+        return r;
+    }
+};
+template <> struct Pack<float> {
+    static constexpr int E = 4;
+    static constexpr unsigned FILL = 0xff800000u;
+    static __device__ __forceinline__ void unpack(u32x4 r, float (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(r[i]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(f[i]);
+        return r;
+    }
+};
+
+// Vector v of a row covers E elements from class v * E on.  The vector that would run over the row's end is moved back to
+// the row's last E elements instead (and so are the vectors behind it): every load is one unconditional 16-byte access
+// inside the row, and drop_repeated() then sets what an earlier vector covers already to -inf, which takes part in nothing.
+template <typename T>
+__device__ __forceinline__ int first_class(int v, int N) {
+    constexpr int E = Pack<T>::E;
+    return min(v * E, max(N - E, 0));
+}
+template <typename T, bool NARROW>
+__device__ __forceinline__ u32x4 ld_row(const T* __restrict__ src, int v, int N) {
+    constexpr int E = Pack<T>::E;
+    if (NARROW && N < E) {                                         // a row shorter than one vector
+        float f[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = e < N ? (float)src[e] : -INFINITY;
+        return Pack<T>::pack(f);                                   // exact: every value is one of T
+    }
+    const unsigned at = (unsigned)first_class<T>(v, N) * (unsigned)sizeof(T);
+    return *reinterpret_cast<const u32x4_a2*>(reinterpret_cast<const unsigned char*>(src) + at);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 drop_repeated(u32x4 r, int v, int N) {
+    constexpr int E = Pack<T>::E;
+    const int repeated = v * E - first_class<T>(v, N);
+    float f[E];
+    Pack<T>::unpack(r, f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = e < repeated ? -INFINITY : f[e];
+    return Pack<T>::pack(f);
+}
+
+__device__ __forceinline__ float ld_as_float(const void* p, long long i, int type) {
+    if (type == DS_BF16) return (float)static_cast<const bf16*>(p)[i];
+    if (type == DS_FP16) return (float)static_cast<const f16*>(p)[i];
+    return static_cast<const float*>(p)[i];
+}
+
+// Workgroup barrier that orders LDS but leaves global loads in flight (a __syncthreads would drain them).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Keeps the packed vector, not its fp32 values, in registers between two passes over a row, and one vector's work from
+// being interleaved with the next one's: both would double the registers of a wide row and spill it.
+__device__ __forceinline__ void hold(u32x4& r) {
+    asm volatile("" : "+v"(r));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The same number, but the compiler does not know: what it derives from it for every vector of one pass (offsets, columns)
+// is then not kept in registers for the next.
+__device__ __forceinline__ int anew(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Running maximum with two sums of exponentials relative to it: st with factor kt = log2(e) / T, s1 with log2(e).
+struct Stat {
+    float m, st, s1;
+};
+template <bool TWO>
+__device__ __forceinline__ Stat merge(Stat a, Stat b, float kt) {
+    Stat r;
+    r.m = fmaxf(a.m, b.m);
+    const float base = finite_or_zero(r.m);
+    r.st = a.st * exp2_fast((a.m - base) * kt) + b.st * exp2_fast((b.m - base) * kt);
+    r.s1 = TWO ? a.s1 * exp2_fast((a.m - base) * DS_LOG2E) + b.s1 * exp2_fast((b.m - base) * DS_LOG2E) : r.st;
+    return r;
+}
+template <bool TWO>
+__device__ __forceinline__ Stat wave_merge(Stat a, float kt) {
+    const float m = wave_max(a.m), base = finite_or_zero(m);
+    a.st = wave_sum(a.st * exp2_fast((a.m - base) * kt));
+    a.s1 = TWO ? wave_sum(a.s1 * exp2_fast((a.m - base) * DS_LOG2E)) : a.st;
+    a.m = m;
+    return a;
+}
+template <bool TWO, int E>
+__device__ __forceinline__ void accumulate(Stat& s, const float (&f)[E], float kt) {
+    float vm = f[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) vm = fmaxf(vm, f[e]);
+    const float m = fmaxf(s.m, vm), base = finite_or_zero(m);
+    const float d0 = s.m - base;
+    float st = s.st * exp2_fast(d0 * kt), s1 = TWO ? s.s1 * exp2_fast(d0 * DS_LOG2E) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float d = f[e] - base;
+        st += exp2_fast(d * kt);
+        if (TWO) s1 += exp2_fast(d * DS_LOG2E);
+    }
+    s.m = m;
+    s.st = st;
+    s.s1 = TWO ? s1 : st;
+}
+
+// ------------------------------------------------------------------------------------------
+// Loss and gradient.  With P the teacher's distribution over the listed classes, q = softmax(z / T) and w = grad_scale / B:
+//   soft = sum_c P_c (log P_c - log q_c)  (+ the same term for the rest of both distributions when an lse is given)
+//   hard = logsumexp(z) - z[label]
+//   row loss = (1 - alpha) hard + alpha T^2 soft
+//   d/dz_i = w (1 - alpha) (softmax(z)_i - [i = label]) + w alpha T (M q_i - P_i)              listed classes, or without an lse
+//                                                       + w alpha T q_i (M q_r - P_r) / q_r    the others, q_r / P_r = the rests
+// with M = sum P + P_r: 1, unless the lse is not that of the teacher's row, or the student has no rest to compare.
+//
+// Wave 0 reads the k slots while every wave's share of the row is on its way: it merges slots of one class (one bit per
+// class in LDS finds them), and the bits also take the listed classes out of the sums of the rest: q_r is a sum of its
+// own and never 1 - (a sum close to 1), relative to the rest's own maximum, so a student that is sure of the listed
+// classes does not underflow it.  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
+// after a barrier wave 0 rewrites the listed classes and the label (k + 1 elements).
+// ------------------------------------------------------------------------------------------
+struct DistillParams {
+    const void* logits;
+    const void* labels;
+    const void* values;
+    const void* indices;
+    const float* lse;
+    void* dlogits;
+    float* row_loss;
+    long long ld_in, ld_val, ld_idx, st_val, st_idx;
+    int B, N, k, ld_out;
+    int label_bytes, index_bytes, value_type;
+    float inv_t, w_soft_grad, w_hard_grad, w_soft_loss, w_hard_loss;
+};
+
+template <typename T, int THREADS, int VPT, bool TWO>
+__global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p) {
+    constexpr int E = Pack<T>::E, W = THREADS / 64;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ Stat part[W + 1];
+    __shared__ float slot_sum;                                     // sum of P, negative: the row has no slots
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, N = p.N, k = p.k;
+    const int nv = (N + E - 1) / E;
+    unsigned* bits = reinterpret_cast<unsigned*>(lds);
+    const int words = ((N + 127) / 128) * 4;                       // a whole number of 16-byte stores
+    int* s_idx = reinterpret_cast<int*>(bits + words);
+    float* s_p = reinterpret_cast<float*>(s_idx + k);
+    float* s_z = s_p + k;
+    float* s_q = s_z + k;
+    const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld_in;
+    T* dst = static_cast<T*>(p.dlogits) + (long long)row * p.ld_out;
+    const float kt = p.inv_t * DS_LOG2E;
+    const bool rest = p.lse != nullptr;
+
+    u32x4 r[VPT > 0 ? VPT : 1];
+    if (VPT > 0) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
+    }
+
+    int label = -1;
+    float z_label = 0.0f;
+    if (p.labels) {
+        const long long l = p.label_bytes == 8 ? static_cast<const long long*>(p.labels)[row]
+                                               : (long long)static_cast<const int*>(p.labels)[row];
+        label = l >= 0 && l < N ? (int)l : -1;
+    }
+    if (wave == 0) {
+        for (int i = lane; i < words / 4; i += 64) reinterpret_cast<u32x4*>(bits)[i] = u32x4{0, 0, 0, 0};
+        bool twice = false;
+        float tmax = -INFINITY;
+        for (int s = lane; s < k; s += 64) {
+            const long long oi = (long long)row * p.ld_idx + s * p.st_idx;
+            const long long li = p.index_bytes == 8 ? static_cast<const long long*>(p.indices)[oi]
+                                                    : (long long)static_cast<const int*>(p.indices)[oi];
+            float t = ld_as_float(p.values, (long long)row * p.ld_val + s * p.st_val, p.value_type);
+            const int i = li >= 0 && li < N && t != -INFINITY ? (int)li : -1;
+            t = i >= 0 ? t * p.inv_t : -INFINITY;
+            if (i >= 0) twice |= (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
+            s_idx[s] = i;
+            s_p[s] = t;
+            s_z[s] = i >= 0 ? (float)src[i] : -INFINITY;
+            tmax = t != t ? t : fmaxf(tmax, t);
+        }
+        if (label >= 0) z_label = (float)src[label];
+        __builtin_amdgcn_wave_barrier();
+        const float top = wave_max(tmax);
+        const bool any = __ballot(tmax != -INFINITY) != 0;         // a NaN counts: it shall reach the loss
+        float total = 0.0f;
+        for (int s = lane; s < k; s += 64) {
+            const float t = s_p[s];
+            const float e = s_idx[s] < 0 ? 0.0f : expf(t - (rest ? p.lse[row] : top));
+            s_p[s] = e;
+            total += e;
+        }
+        total = wave_sum(total);
+        if (!rest && any) {
+            const float inv = 1.0f / total;
+            for (int s = lane; s < k; s += 64) s_p[s] *= inv;
+            total = 1.0f + (total - total);                        // 1, or NaN
+        }
+        if (__ballot(twice)) {                                     // slots of one class: the first takes the sum, in slot order
+            __builtin_amdgcn_wave_barrier();
+            for (int s = lane; s < k; s += 64) {
+                const int i = s_idx[s];
+                float sum = 0.0f;
+                bool first = i >= 0;
+                for (int o = 0; o < k; ++o)
+                    if (s_idx[o] == i) {
+                        first &= o >= s;
+                        sum += s_p[o];
+                    }
+                s_q[s] = first ? sum : -1.0f;
+            }
+            __builtin_amdgcn_wave_barrier();
+            for (int s = lane; s < k; s += 64) {
+                if (s_q[s] == -1.0f) s_idx[s] = -1;
+                s_p[s] = s_q[s] == -1.0f ? 0.0f : s_q[s];
+            }
+        }
+        Stat own = {-INFINITY, 0.0f, 0.0f};
+        if (rest)                                                  // the rest's sums skip the listed classes: theirs come from here
+            for (int s = lane; s < k; s += 64) {
+                const float f[1] = {s_idx[s] >= 0 ? s_z[s] : -INFINITY};
+                accumulate<TWO, 1>(own, f, kt);
+            }
+        own = wave_merge<TWO>(own, kt);
+        if (lane == 0) {
+            part[W] = own;
+            slot_sum = any ? total : -1.0f;
+        }
+    }
+    if (rest) lds_barrier();                                       // the bits are complete
+
+    Stat mine = {-INFINITY, 0.0f, 0.0f};
+    // -inf for what this vector repeats of an earlier one and, with a rest, for the listed classes
+    auto take_out = [&](u32x4 q, int v, bool whole) -> u32x4 {
+        if (!whole) q = drop_repeated<T>(q, v, N);
+        if (rest) {
+            const int c = first_class<T>(v, N);
+            unsigned b = bits[c >> 5] >> (c & 31);
+            if ((c & 31) > 32 - E) b |= bits[(c >> 5) + 1] << (32 - (c & 31));
+            b &= (1u << E) - 1u;
+            if (b) {
+                float f[E];
+                Pack<T>::unpack(q, f);
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] = (b >> e) & 1u ? -INFINITY : f[e];
+                q = Pack<T>::pack(f);
+            }
+        }
+        return q;
+    };
+    if (VPT > 0) {
+        const int t = anew(tid);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            r[j] = take_out(r[j], j * THREADS + t, (j + 1) * THREADS * E <= N);
+            float f[E];
+            Pack<T>::unpack(r[j], f);
+            accumulate<TWO, E>(mine, f, kt);
+            hold(r[j]);
+        }
+    } else {
+        for (int v = tid; v < nv; v += 4 * THREADS) {
+            u32x4 q[4];
+            const bool whole = (long long)(v - tid + 4 * THREADS) * E <= N;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = ld_row<T, false>(src, v + u * THREADS, N);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float f[E];
+                Pack<T>::unpack(take_out(q[u], v + u * THREADS, whole), f);
+                accumulate<TWO, E>(mine, f, kt);
+            }
+        }
+    }
+    mine = wave_merge<TWO>(mine, kt);
+    if (lane == 0) part[wave] = mine;
+    lds_barrier();
+
+    // every wave works out the row's numbers for itself
+    Stat a = part[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) a = merge<TWO>(a, part[w], kt);
+    const Stat all = rest ? merge<TWO>(a, part[W], kt) : a;
+    const float m = all.m;
+    const bool some = m != -INFINITY || all.st != all.st;          // a row of -inf has no distribution: it counts for nothing
+    const float sum_p = slot_sum;
+    const bool soft = some && !(sum_p < 0.0f);
+    const float base = finite_or_zero(a.m);
+    const float inv_st = some ? 1.0f / all.st : 0.0f, inv_s1 = some ? 1.0f / all.s1 : 0.0f;
+    const float p_rest = fmaxf(1.0f - sum_p, 0.0f);
+    const float q_rest = rest ? a.st * exp2_fast((a.m - m) * kt) * inv_st : 0.0f;
+    const bool has_rest = rest && a.st > 0.0f;                     // nothing outside the list: no rest to compare
+    const float mass = sum_p + (has_rest ? p_rest : 0.0f);
+    float ct = 0.0f;
+    if (soft) ct = rest ? (has_rest ? p.w_soft_grad * (mass * q_rest - p_rest) / a.st : 0.0f) : p.w_soft_grad * mass * inv_st;
+    const bool has_label = label >= 0 && some;
+    const float wh = has_label ? p.w_hard_grad : 0.0f;
+    const float c1 = has_label ? wh * inv_s1 * (rest ? exp2_fast((a.m - m) * DS_LOG2E) : 1.0f) : 0.0f;   // (an empty row: m is -inf)
+    const float cs = ct + c1;                                      // T = 1: one exponential serves both
+
+    auto gradient = [&](u32x4 q, int v, bool whole) {
+        float f[E], g[E];
+        Pack<T>::unpack(q, f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = f[e] - base;
+            g[e] = TWO ? ct * exp2_fast(d * kt) + c1 * exp2_fast(d * DS_LOG2E) : cs * exp2_fast(d * kt);
+        }
+        if (whole || (v + 1) * E <= N) {
+            __builtin_nontemporal_store(Pack<T>::pack(g),
+                                        reinterpret_cast<u32x4*>(reinterpret_cast<unsigned char*>(dst) + (unsigned)v * 16u));
+        } else {
+            const int c = first_class<T>(v, N), repeated = v * E - c;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e >= repeated && c + e < N) dst[c + e] = (T)g[e];
+        }
+    };
+    if (VPT > 0) {
+        const int t = anew(tid);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            gradient(r[j], j * THREADS + t, (j + 1) * THREADS * E <= N);
+            hold(r[j]);
+        }
+    } else {
+        for (int v = tid; v < nv; v += 4 * THREADS) {
+            u32x4 q[4];
+            const bool whole = (long long)(v - tid + 4 * THREADS) * E <= N;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = ld_row<T, false>(src, v + u * THREADS, N);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) gradient(take_out(q[u], v + u * THREADS, whole), v + u * THREADS, whole);
+        }
+    }
+    for (int c = N + tid; c < p.ld_out; c += THREADS) dst[c] = (T)0.0f;   // the padding, whatever the row holds
+    __syncthreads();                                               // the row is written: now the elements that differ
+    if (wave != 0) return;
+    float loss = 0.0f;
+    const float log_st = some ? logf(all.st) : 0.0f;
+    bool label_listed = false;
+    for (int s = lane; s < k; s += 64) {
+        const int i = s_idx[s];
+        if (i < 0) continue;
+        const float P = s_p[s], d = s_z[s] - finite_or_zero(m);
+        if (soft && !(P == 0.0f)) loss += P * (logf(P) - (d * p.inv_t - log_st));
+        float g = soft ? p.w_soft_grad * (mass * exp2_fast(d * kt) * inv_st - P) : 0.0f;
+        g += wh * (exp2_fast(d * DS_LOG2E) * inv_s1 - (i == label ? 1.0f : 0.0f));
+        dst[i] = (T)g;
+        label_listed |= i == label;
+    }
+    loss = wave_sum(loss);
+    label_listed = __ballot(label_listed) != 0;
+    if (lane == 0) {
+        if (soft && has_rest && p_rest > 0.0f)
+            loss += p_rest * (logf(p_rest) - ((a.m - m) * p.inv_t + logf(a.st) - log_st));
+        loss *= p.w_soft_loss;
+        if (has_label) {
+            if (!label_listed) {
+                const float d = z_label - base;
+                const float g = ct * exp2_fast(d * kt) + wh * (exp2_fast((z_label - m) * DS_LOG2E) * inv_s1 - 1.0f);
+                dst[label] = (T)g;
+            }
+            if (p.w_hard_loss != 0.0f) loss += p.w_hard_loss * (logf(all.s1) + (m - z_label));
+        }
+        p.row_loss[row] = loss;
+    }
+}
+
+// Mean of the row losses in a fixed order: the same bits from run to run.
+__global__ __launch_bounds__(256) void distill_mean_kernel(const float* __restrict__ v, float* __restrict__ out, int n) {
+    __shared__ double red[256];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) s += (double)v[i];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int w = 128; w > 0; w >>= 1) {
+        if (threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *out = n > 0 ? (float)(red[0] / (double)n) : 0.0f;
+}
+
+template <typename T, bool TWO>
+static void launch_distill(const DistillParams& p, hipStream_t s) {
+    const int nv = (p.N + Pack<T>::E - 1) / Pack<T>::E;
+    const size_t shared = (size_t)((p.N + 127) / 128) * 16 + (size_t)p.k * 16;
+    const dim3 grid(p.B);
+#define DS_LAUNCH(TH, V) hipLaunchKernelGGL((distill_kernel<T, TH, V, TWO>), grid, dim3(TH), shared, s, p)
+    if (nv <= 64) DS_LAUNCH(64, 1);
+    else if (nv <= 128) DS_LAUNCH(64, 2);
+    else if (nv <= 256) DS_LAUNCH(64, 4);
+    else if (nv <= 1024) DS_LAUNCH(256, 4);
+    else if (nv <= 4096) DS_LAUNCH(1024, 4);
+    else if (nv <= 8192) DS_LAUNCH(1024, 8);
+    else DS_LAUNCH(1024, 0);
+#undef DS_LAUNCH
+}
+
+// Status -1: an argument outside what the kernel is built for (nothing was launched).
+PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* values, const void* indices, const void* lse,
+                           void* dlogits, void* row_loss, void* loss, int B, int N, int k, long long ld_in, long long ld_val,
+                           long long st_val, long long ld_idx, long long st_idx, int ld_out, int type, int value_type,
+                           int label_bytes, int index_bytes, float temperature, float alpha, float grad_scale,
+                           hipStream_t s) {
+    if (B < 0 || N < 1 || N > DS_MAX_CLASSES || k < 1 || k > DS_MAX_K || ld_out < N || ld_out % 64 != 0) return -1;
+    if (type < 0 || type > 2 || value_type < 0 || value_type > 2 || (label_bytes != 4 && label_bytes != 8)) return -1;
+    if ((index_bytes != 4 && index_bytes != 8) || !(temperature > 0.0f)) return -1;
+    if (B > 0) {
+        DistillParams p;
+        p.logits = logits, p.labels = labels, p.values = values, p.indices = indices;
+        p.lse = static_cast<const float*>(lse);
+        p.dlogits = dlogits, p.row_loss = static_cast<float*>(row_loss);
+        p.ld_in = ld_in, p.ld_val = ld_val, p.ld_idx = ld_idx, p.st_val = st_val, p.st_idx = st_idx;
+        p.B = B, p.N = N, p.k = k, p.ld_out = ld_out;
+        p.label_bytes = label_bytes, p.index_bytes = index_bytes, p.value_type = value_type;
+        p.inv_t = 1.0f / temperature;
+        p.w_soft_loss = alpha * temperature * temperature;
+        p.w_hard_loss = labels ? 1.0f - alpha : 0.0f;
+        p.w_soft_grad = alpha * temperature * grad_scale / (float)B;
+        p.w_hard_grad = p.w_hard_loss * grad_scale / (float)B;
+        const bool two = p.w_hard_loss != 0.0f && temperature != 1.0f;
+        if (type == DS_BF16) two ? launch_distill<bf16, true>(p, s) : launch_distill<bf16, false>(p, s);
+        else if (type == DS_FP16) two ? launch_distill<f16, true>(p, s) : launch_distill<f16, false>(p, s);
+        else two ? launch_distill<float, true>(p, s) : launch_distill<float, false>(p, s);
+        const int rc = pdt_launch_status();
+        if (rc != 0) return rc;
+    }
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(256), 0, s, (const float*)row_loss, (float*)loss, B);
+    return pdt_launch_status();
+}
+
+// ------------------------------------------------------------------------------------------
+// The k largest logits of a row in falling order (ties: lower class first; a NaN before every number; classes at -inf
+// never) and the row's logsumexp at temperature T.
+//
+// A lower bound of the k-th largest comes from the threads' own maxima: with W waves, the smallest over the waves of the
+// ceil(k / W)-th largest lane maximum has at least k elements at or above it, and for values in no particular order only
+// a few times k.  Those candidates go to LDS as 64-bit keys (value, then class) and are sorted there; the keys differ, so
+// the order in which the candidates arrive does not matter.  Rows on which the bound is too low (many equal values,
+// sorted rows) are cut to exactly k candidates by bisecting the value and, among equals, the class: exact, some 50
+// passes over the registers.
+// ------------------------------------------------------------------------------------------
+struct TopParams {
+    const void* logits;
+    void* values;
+    int* indices;
+    float* lse;
+    long long ld_in;
+    int N, k;
+    float inv_t;
+};
+
+// unsigned order = float order; -0 = +0, NaN on top
+__device__ __forceinline__ unsigned order_key(float f) {
+    if (f != f) return 0xffffffffu;
+    const unsigned u = __float_as_uint(f + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long slot_key(float f, int c) {
+    return (unsigned long long)order_key(f) << 32 | (unsigned)~c;
+}
+__device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v, int mask) {
+    const unsigned lo = __shfl_xor((unsigned)v, mask, 64), hi = __shfl_xor((unsigned)(v >> 32), mask, 64);
+    return (unsigned long long)hi << 32 | lo;
+}
+
+template <typename T, int THREADS, int VPT>
+__global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) {
+    constexpr int E = Pack<T>::E, W = THREADS / 64, CAP = THREADS == 64 ? 512 : 2048;
+    __shared__ unsigned long long cand[CAP];
+    __shared__ Stat part[W];
+    __shared__ float bound[W];
+    __shared__ int tally[W];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, N = p.N, k = p.k;
+    const int nv = (N + E - 1) / E;
+    const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld_in;
+    const float kt = p.inv_t * DS_LOG2E;
+
+    u32x4 r[VPT > 0 ? VPT : 1];
+    if (VPT > 0) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
+    }
+    if (VPT > 0) {
+        const int t = anew(tid);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if ((j + 1) * THREADS * E > N) r[j] = drop_repeated<T>(r[j], j * THREADS + t, N);
+    }
+    auto over_row = [&](auto&& fn) {                               // fn(values, first class) for every vector of this thread
+        if (VPT > 0) {
+            const int t = anew(tid);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                float f[E];
+                Pack<T>::unpack(r[j], f);
+                fn(f, first_class<T>(j * THREADS + t, N));
+                hold(r[j]);
+            }
+        } else {
+            for (int v = tid; v < nv; v += 4 * THREADS) {
+                u32x4 q[4];
+                const bool whole = (long long)(v - tid + 4 * THREADS) * E <= N;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) q[u] = ld_row<T, false>(src, v + u * THREADS, N);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float f[E];
+                    Pack<T>::unpack(whole ? q[u] : drop_repeated<T>(q[u], v + u * THREADS, N), f);
+                    fn(f, first_class<T>(v + u * THREADS, N));
+                }
+            }
+        }
+    };
+    auto keep = [&](float f, int c) {
+        const int at = atomicAdd(&count, 1);
+        if (at < CAP) cand[at] = slot_key(f, c);
+    };
+
+    Stat mine = {-INFINITY, 0.0f, 0.0f};
+    over_row([&](const float (&f)[E], int) { accumulate<false, E>(mine, f, kt); });
+    float v = mine.m;                                              // sorted over the wave, falling
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            const float o = __shfl_xor(v, step, 64);
+            v = ((lane & step) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
+        }
+    const float low = __shfl(v, (k + W - 1) / W - 1, 64);
+    mine = wave_merge<false>(mine, kt);
+    if (lane == 0) {
+        bound[wave] = low;
+        part[wave] = mine;
+    }
+    if (tid == 0) count = 0;
+    lds_barrier();
+    float floor_v = bound[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) floor_v = fminf(floor_v, bound[w]);
+    if (tid == 0) {
+        Stat a = part[0];
+        for (int w = 1; w < W; ++w) a = merge<false>(a, part[w], kt);
+        p.lse[row] = finite_or_zero(a.m) * p.inv_t + logf(a.st);
+    }
+    over_row([&](const float (&f)[E], int c) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) any |= !(f[e] < floor_v);      // NaN too
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (!(f[e] < floor_v) && f[e] != -INFINITY) keep(f[e], c + e);
+        }
+    });
+    lds_barrier();
+    int n = count;
+
+    if (n > CAP) {                                                 // the bound was too low for this row
+        auto total = [&](int mine_n) {
+            const int t = (int)wave_sum((float)mine_n);            // below 2^24: exact
+            lds_barrier();                                         // the last round's tallies have been read
+            if (lane == 0) tally[wave] = t;
+            lds_barrier();
+            int s = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += tally[w];
+            return s;
+        };
+        unsigned t = 0;                                            // largest key that k elements reach
+        for (int b = 31; b >= 0; --b) {
+            const unsigned c = t | 1u << b;
+            int m = 0;
+            over_row([&](const float (&f)[E], int) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) m += f[e] != -INFINITY && order_key(f[e]) >= c;
+            });
+            if (total(m) >= k) t = c;
+        }
+        int above = 0;
+        over_row([&](const float (&f)[E], int) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) above += f[e] != -INFINITY && order_key(f[e]) > t;
+        });
+        const int need = k - total(above);
+        int lo = 0, hi = N - 1;                                    // smallest class up to which `need` elements equal the key
+        while (lo < hi) {
+            const int mid = lo + (hi - lo) / 2;
+            int m = 0;
+            over_row([&](const float (&f)[E], int c) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) m += f[e] != -INFINITY && order_key(f[e]) == t && c + e <= mid;
+            });
+            if (total(m) >= need) hi = mid;
+            else lo = mid + 1;
+        }
+        lds_barrier();
+        if (tid == 0) count = 0;
+        lds_barrier();
+        over_row([&](const float (&f)[E], int c) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const unsigned key = order_key(f[e]);
+                if (f[e] != -INFINITY && (key > t || (key == t && c + e <= lo))) keep(f[e], c + e);
+            }
+        });
+        lds_barrier();
+        n = count;
+    }
+
+    T* values = static_cast<T*>(p.values) + (long long)row * k;
+    int* indices = p.indices + (long long)row * k;
+    auto put = [&](int s, unsigned long long key, bool filled) {
+        const int c = (int)~(unsigned)key;
+        values[s] = filled ? src[c] : (T)-INFINITY;
+        indices[s] = filled ? c : -1;
+    };
+    if (n <= 64) {                                                 // one wave, in registers
+        if (wave != 0) return;
+        unsigned long long key = lane < n ? cand[lane] : 0ull;
+#pragma unroll
+        for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+            for (int step = size >> 1; step > 0; step >>= 1) {
+                const unsigned long long o = shfl_xor_u64(key, step);
+                const bool take_max = ((lane & step) == 0) == ((lane & size) == 0);
+                key = (key > o) == take_max ? key : o;
+            }
+        for (int s = lane; s < k; s += 64) put(s, key, s == lane && s < n);
+        return;
+    }
+    int size2 = 128;
+    while (size2 < n) size2 <<= 1;
+    for (int i = n + tid; i < size2; i += THREADS) cand[i] = 0ull;
+    lds_barrier();
+    for (int size = 2; size <= size2; size <<= 1)
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            for (int i = tid; i < size2 / 2; i += THREADS) {
+                const int a = 2 * i - (i & (step - 1)), b = a + step;
+                const unsigned long long x = cand[a], y = cand[b];
+                if ((x < y) == ((a & size) == 0)) {
+                    cand[a] = y;
+                    cand[b] = x;
+                }
+            }
+            lds_barrier();
+        }
+    for (int s = tid; s < k; s += THREADS) put(s, cand[s], s < n);
+}
+
+template <typename T>
+static void launch_top(const TopParams& p, int B, hipStream_t s) {
+    const int nv = (p.N + Pack<T>::E - 1) / Pack<T>::E;
+#define DS_LAUNCH(TH, V) hipLaunchKernelGGL((top_logits_kernel<T, TH, V>), dim3(B), dim3(TH), 0, s, p)
+    // at least two threads per wanted logit: with fewer the bound from the thread maxima lets too many candidates pass
+    if (nv <= 64 && p.k <= 32) DS_LAUNCH(64, 1);
+    else if (nv <= 128 && p.k <= 32) DS_LAUNCH(64, 2);
+    else if (nv <= 256 && p.k <= 32) DS_LAUNCH(64, 4);
+    else if (nv <= 1024 && p.k <= 128) DS_LAUNCH(256, 4);
+    else if (nv <= 4096) DS_LAUNCH(1024, 4);
+    else if (nv <= 8192) DS_LAUNCH(1024, 8);
+    else DS_LAUNCH(1024, 0);
+#undef DS_LAUNCH
+}
+
+// Status -1: an argument outside what the kernel is built for (nothing was launched).
+PDT_API int pdt_top_logits(const void* logits, void* values, void* indices, void* lse, int B, int N, int k, long long ld_in,
+                           int type, float temperature, hipStream_t s) {
+    if (B < 0 || N < 1 || k < 1 || k > DS_MAX_K || k > N || N > (1 << 24) || type < 0 || type > 2 || !(temperature > 0.0f))
+        return -1;
+    if (B == 0) return 0;
+    TopParams p;
+    p.logits = logits, p.values = values, p.indices = static_cast<int*>(indices), p.lse = static_cast<float*>(lse);
+    p.ld_in = ld_in, p.N = N, p.k = k, p.inv_t = 1.0f / temperature;
+    if (type == DS_BF16) launch_top<bf16>(p, B, s);
+    else if (type == DS_FP16) launch_top<f16>(p, B, s);
+    else launch_top<float>(p, B, s);
+    return pdt_launch_status();
+}

@@ -16,6 +16,7 @@ import torch
 
 from . import build as _build
 from .ref import MASK_NONE, MASK_RECOMPUTE, MASK_TENSOR  # noqa: F401  (re-exported)
+from .ref import check_distill_ce, check_top_logits
 
 name = "hip"
 # conv_dgrad reads the transposed copies ``wt`` only: the forward weights may be updated while backward still runs
@@ -95,6 +96,9 @@ _sig("pdt_bnfold_scale_weights", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
 _sig("pdt_bnfold_prepare", _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _i, _vp)
 _sig("pdt_bnfold_wgrad", _vp, _vp, _vp, _vp, _f, _vp, _vp, _i, _i, _vp)
 _sig("pdt_bnfold_sums", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp)
+_sig("pdt_distill_ce", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _i, _i, _f, _f,
+     _f, _vp)
+_sig("pdt_top_logits", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _f, _vp)
 _sig("pdt_set_deterministic", _i)
 _sig("pdt_accumulator_rows")
 
@@ -1262,6 +1266,50 @@ def ce_metrics(logits, labels):
     rc = _lib.pdt_ce_metrics(_p(logits), _p(labels.contiguous()), _p(out), B, N, logits.stride(0), _stream())
     _check(rc, "pdt_ce_metrics")
     return out
+
+
+# --------------------------------------------------------------------------- distillation
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _here(what: str, *tensors) -> None:
+    """Kernels run on the current device's current stream: operands elsewhere are an error, not a wild read."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != cur):
+            raise ValueError(f"{what}: operand on {t.device}, but the current device is cuda:{cur}")
+
+
+def top_logits(logits, k: int, temperature: float = 1.0):
+    check_top_logits(logits, k, temperature)
+    _here("top_logits", logits)
+    B, N = logits.shape
+    dev = logits.device
+    values = torch.empty(B, k, dtype=logits.dtype, device=dev)
+    indices = torch.empty(B, k, dtype=torch.int32, device=dev)
+    lse = torch.empty(B, dtype=torch.float32, device=dev)
+    rc = _lib.pdt_top_logits(logits.data_ptr(), values.data_ptr(), indices.data_ptr(), lse.data_ptr(), B, N, k, logits.stride(0),
+                             _LOGIT_TYPES[logits.dtype], temperature, _stream())
+    _check(rc, "pdt_top_logits")
+    return values, indices, lse
+
+
+def distill_ce(logits, labels, values, indices, temperature: float = 1.0, alpha: float = 0.5, lse=None,
+               grad_scale: float = 1.0):
+    check_distill_ce(logits, labels, values, indices, temperature, alpha, lse)
+    _here("distill_ce", logits, labels, values, indices, lse)
+    B, N = logits.shape
+    ld_out, dev = _npad(N), logits.device
+    dlog = torch.empty(B, ld_out, dtype=logits.dtype, device=dev)
+    losses = torch.empty(B + 1, dtype=torch.float32, device=dev)      # the mean, then the rows' own
+    at = losses.data_ptr()
+    rc = _lib.pdt_distill_ce(logits.data_ptr(), _p(labels), values.data_ptr(), indices.data_ptr(), _p(lse), dlog.data_ptr(), at + 4, at,
+                             B, N, values.shape[1], logits.stride(0), values.stride(0), values.stride(1), indices.stride(0),
+                             indices.stride(1), ld_out, _LOGIT_TYPES[logits.dtype], _LOGIT_TYPES[values.dtype],
+                             8 if labels is None else labels.element_size(), indices.element_size(), temperature, alpha,
+                             grad_scale, _stream())
+    _check(rc, "pdt_distill_ce")
+    return losses[0], dlog[:, :N]
 
 
 # --------------------------------------------------------------------------- optimizer

@@ -535,6 +535,126 @@ def ce_metrics(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     return torch.stack([loss_sum, (rank < 1).sum().float(), (rank < 5).sum().float(), n])
 
 
+# ---------------------------------------------------------------------------- distillation
+MAX_TOP = 512                # slots per row
+MAX_CLASSES = 262144
+_LOGIT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _check_logits(what: str, logits: torch.Tensor, temperature: float) -> None:
+    if logits.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"{what}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_CLASSES:
+        raise ValueError(f"{what}: logits must be [rows, classes] with 1 to {MAX_CLASSES} classes, got {tuple(logits.shape)}")
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError(f"{what}: logits must have unit column stride")
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError(f"{what}: temperature must lie in [0.001, 1000], got {temperature}")
+
+
+def check_top_logits(logits: torch.Tensor, k: int, temperature: float) -> None:
+    _check_logits("top_logits", logits, temperature)
+    if not 1 <= k <= min(MAX_TOP, logits.shape[1]):
+        raise ValueError(f"top_logits: k must lie in [1, {min(MAX_TOP, logits.shape[1])}], got {k}")
+
+
+def check_distill_ce(logits, labels, values, indices, temperature: float, alpha: float, lse) -> None:
+    _check_logits("distill_ce", logits, temperature)
+    B = logits.shape[0]
+    if values.dtype not in _LOGIT_DTYPES or indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"distill_ce: values must be bf16 / fp16 / fp32 and indices int32 / int64, got {values.dtype}, {indices.dtype}")
+    if values.dim() != 2 or values.shape[0] != B or values.shape != indices.shape or not 1 <= values.shape[1] <= MAX_TOP:
+        raise ValueError(f"distill_ce: values and indices must both be [{B}, k] with k in [1, {MAX_TOP}], got "
+                         f"{tuple(values.shape)}, {tuple(indices.shape)}")
+    if labels is not None:
+        if labels.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"distill_ce: labels must be int32 / int64, got {labels.dtype}")
+        if labels.shape != (B,) or (B > 1 and labels.stride(0) != 1):
+            raise ValueError(f"distill_ce: labels must be [{B}] and contiguous, got {tuple(labels.shape)}")
+    if lse is not None:
+        if lse.dtype != torch.float32:
+            raise TypeError(f"distill_ce: lse must be fp32, got {lse.dtype}")
+        if lse.shape != (B,) or (B > 1 and lse.stride(0) != 1):
+            raise ValueError(f"distill_ce: lse must be [{B}] and contiguous, got {tuple(lse.shape)}")
+    if not 0.0 <= alpha <= 1.0:
+        raise ValueError(f"distill_ce: alpha must lie in [0, 1], got {alpha}")
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
+    """What a teacher hands to :func:`distill_ce`: ``(values[B, k], indices[B, k] int32, lse[B] fp32)``.
+
+    The ``k`` largest logits of each row in falling order, ties to the lower class, a NaN before every number; a class at
+    ``-inf`` is never chosen (slots left over hold value ``-inf``, class ``-1``).  ``lse`` is ``logsumexp(logits / T)`` over the
+    whole row (``-inf`` for a row that is ``-inf`` throughout).  ``logits``: bf16, fp16 or fp32, unit column stride, any row
+    stride; up to ``MAX_TOP`` slots and ``MAX_CLASSES`` classes."""
+    check_top_logits(logits, k, temperature)
+    l32 = logits.float()
+    order = torch.where(l32.isnan(), torch.full_like(l32, torch.inf), l32)
+    # a NaN sorts before +inf: two stable passes, the second by "is a NaN"
+    idx = torch.sort(order, dim=1, descending=True, stable=True).indices
+    nan_first = torch.sort(l32.gather(1, idx).isnan().to(torch.uint8), dim=1, descending=True, stable=True).indices
+    idx = idx.gather(1, nan_first)[:, :k]
+    values = logits.gather(1, idx)
+    idx = torch.where(values == -torch.inf, torch.full_like(idx, -1), idx)
+    return values, idx.to(torch.int32), torch.logsumexp(l32 / temperature, dim=1)
+
+
+def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: torch.Tensor, indices: torch.Tensor,
+               temperature: float = 1.0, alpha: float = 0.5, lse: Optional[torch.Tensor] = None, grad_scale: float = 1.0):
+    """Distillation from a teacher's top logits: mean loss and its gradient in one pass.
+
+    A row's loss is ``(1 - alpha) * hard + alpha * T^2 * soft``.  ``hard`` is the cross-entropy with ``labels`` (None: left out),
+    ``soft`` the divergence KL(P || q) of ``q = softmax(logits / T)`` from the teacher's ``P``: ``exp(values / T - L)`` at the classes
+    ``indices``.  With ``lse`` (the teacher's logsumexp at ``T``, see :func:`top_logits`) ``L = lse`` and what either distribution has
+    outside the listed classes is compared as one class more; without it ``L`` is the logsumexp over the slots, and ``P`` sums to 1
+    over them.  The gradient is that of ``grad_scale * loss``, in the logits' type (on the GPU: in rows padded to a multiple of 64
+    columns, the padding zero, as ``linear_bwd`` takes them).
+
+    Left out of the mean's numerator, never of its ``B``: the hard term of a row whose label is no class, the soft term of a row
+    without slots, everything of a row whose logits are all ``-inf``.  A slot is empty if its index is no class or its value is
+    ``-inf``; slots of one class are added up.  Where the student has nothing outside the listed classes there is no rest to
+    compare.  NaN and +inf in the logits or in a slot that counts reach the loss."""
+    check_distill_ce(logits, labels, values, indices, temperature, alpha, lse)
+    B, N = logits.shape
+    l32 = logits.float()
+    if B == 0:
+        return torch.zeros((), device=logits.device), torch.zeros_like(logits)
+    some = ~(l32 == -torch.inf).all(dim=1, keepdim=True)
+    l32 = torch.where(some, l32, torch.zeros_like(l32))
+    idx = indices.long()
+    filled = (idx >= 0) & (idx < N) & (values != -torch.inf)
+    taught = filled.any(dim=1, keepdim=True) & some
+    t = torch.where(filled, values.float() / temperature, torch.full_like(values, -torch.inf, dtype=torch.float32))
+    total = lse.float()[:, None] if lse is not None else torch.logsumexp(t, dim=1, keepdim=True)
+    p = torch.where(filled, torch.exp(t - total), torch.zeros_like(t))
+    at = torch.where(filled, idx, torch.full_like(idx, N))                    # one column more: a bin for empty slots
+    P = torch.zeros(B, N + 1, device=l32.device).scatter_add_(1, at, p)[:, :N]
+    log_q = torch.log_softmax(l32 / temperature, dim=1)
+    q = log_q.exp()
+    soft = torch.where(P == 0, torch.zeros_like(P), P * (P.log() - log_q)).sum(dim=1, keepdim=True)
+    mass = P.sum(dim=1, keepdim=True)
+    g = mass * q - P
+    if lse is not None:
+        listed = torch.zeros(B, N + 1, dtype=torch.bool, device=l32.device).scatter_(1, at, True)[:, :N]
+        log_r = torch.logsumexp(torch.where(listed, torch.full_like(log_q, -torch.inf), log_q), dim=1, keepdim=True)
+        p_r = (1.0 - mass).clamp_min(0.0)
+        has = log_r != -torch.inf
+        mass = mass + torch.where(has, p_r, torch.zeros_like(p_r))
+        soft = soft + torch.where(has & (p_r > 0), p_r * (p_r.log() - log_r), torch.zeros_like(p_r))
+        g = torch.where(listed, mass * q - P, torch.where(has, mass * q - p_r * torch.exp(log_q - log_r), torch.zeros_like(q)))
+    loss = torch.where(taught, alpha * temperature * temperature * soft, torch.zeros_like(soft))
+    d = torch.where(taught, alpha * temperature * g, torch.zeros_like(g))
+    if labels is not None and alpha != 1.0:
+        lab = labels.long()[:, None]
+        known = (lab >= 0) & (lab < N) & some
+        lab = torch.where(known, lab, torch.zeros_like(lab))
+        logp = torch.log_softmax(l32, dim=1)
+        loss = loss + torch.where(known, -(1.0 - alpha) * logp.gather(1, lab), torch.zeros_like(loss))
+        h = logp.exp().scatter_add_(1, lab, torch.full_like(loss, -1.0))
+        d = d + torch.where(known, (1.0 - alpha) * h, torch.zeros_like(h))
+    return loss.mean(), (d * (grad_scale / B)).to(logits.dtype)
+
+
 # ---------------------------------------------------------------------------- optimizer
 def sgd_step(p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, pc: Optional[torch.Tensor], lr: float,
              momentum: float, weight_decay: float, grad_scale: float, nesterov: bool = False,
