@@ -37,7 +37,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpdt_hip.so")
 ARCH = "gfx950"
 SOURCES = ["elementwise.hip", "reduce.hip", "conv_igemm.hip", "conv_dma.hip", "conv_wgrad.hip", "bn_fold.hip",
-           "xgmi_allreduce.hip", "distill.hip"]
+           "xgmi_allreduce.hip", "distill.hip", "linear.hip"]
 # packed fp32 arithmetic is switched off: some forms of those instructions have given wrong results on this part
 FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-fno-gpu-rdc", "-Wno-unused-result",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -1,0 +1,694 @@
+// Matrix products of a classifier / MLP head with everything around them in the epilogue, bf16 in, fp32 accumulation on
+// the matrix cores (v_mfma_f32_16x16x32_bf16), each result rounded to bf16 once:
+//
+//   forward     z = a w^T + bias,  y = act(z) + residual          a [M][K], w [N][K]
+//   gradients   da = dz w,  dw = dz^T a,  dbias = column sums of dz,  dz = dy act'(z)
+//
+// One tile kernel serves the three products.  An operand is either K-contiguous (its reduction index is the fast one: a and w
+// forward, dz for da) or K-strided (w for da, dz and a for dw); both are staged as they lie in memory by LDS-DMA
+// (buffer_load ... lds, no staging registers) and differ in how fragments are read back: ds_read_b128 for the first,
+// the transposing ds_read_b64_tr_b16 for the second.  No operand is ever transposed in memory.
+#include "common.h"
+
+#define LIN_NONE 0
+#define LIN_RELU 1
+#define LIN_GELU 2
+#define LIN_SILU 3
+
+#define OUT_BF16 0       // epilogue, bf16
+#define OUT_ADD 1        // fp32, added to what is there (gradient buffers)
+#define OUT_PART 2       // fp32 partial sums of one K range, joined by linear_join_kernel
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+typedef u32x4 __attribute__((aligned(2))) u32x4_a2;           // global memory takes unaligned vector accesses
+typedef u32x2 __attribute__((aligned(2))) u32x2_a2;
+typedef __attribute__((address_space(3))) void lin_lds_void_t;
+
+// ------------------------------------------------------------------------------------------ activations
+// Phi(-|z|) of the normal distribution, Abramowitz & Stegun 7.1.26 (|error| < 7.5e-8) with the factor exp(-z^2 / 2) kept
+// apart: the tail falls off as it should (1 % off at z = -9) instead of ending in the rounding of 1 + erf, and the exponential
+// also is the density that the derivative needs.
+__device__ __forceinline__ float normal_tail(float z, float& density) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    const float e = __builtin_amdgcn_exp2f(-x * x * 1.44269504088896341f);
+    density = e * 0.39894228040143268f;
+    return 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+}
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+}
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == LIN_RELU) return z < 0.0f ? 0.0f : z;          // a NaN stays one
+    if (act == LIN_GELU) {
+        float d;
+        const float h = normal_tail(z, d);
+        if (z == -INFINITY) return 0.0f;                       // (0 times infinity)
+        return z > 0.0f ? z * (1.0f - h) : z * h;
+    }
+    if (act == LIN_SILU) return z == -INFINITY ? 0.0f : z * sigmoid(z);
+    return z;
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == LIN_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    if (act == LIN_GELU) {
+        float d;
+        const float h = normal_tail(z, d);
+        if (fabsf(z) == INFINITY) return z > 0.0f ? 1.0f : 0.0f;
+        return (z > 0.0f ? 1.0f - h : h) + z * d;
+    }
+    if (act == LIN_SILU) {
+        const float s = sigmoid(z);
+        return z == -INFINITY ? 0.0f : (z == INFINITY ? 1.0f : s * (1.0f + z * (1.0f - s)));
+    }
+    return 1.0f;
+}
+
+// ------------------------------------------------------------------------------------------ epilogue
+struct Epilogue {
+    void* out;
+    bf16* z;                   // pre-activation, or null
+    const float* bias;         // [N], or null
+    const bf16* res;           // [M][ldr], or null
+    float* ws;                 // OUT_PART: slabs [splits][M][N]
+    long long ldr;
+    int ldo, n_pad;            // row stride of out and z; columns N .. n_pad - 1 are written as zeros
+    int M, N, mode, act, vec;  // vec: rows of out (and z) allow stores of 8 values
+};
+
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    const bf16x2 p = __builtin_convertvector((f32x2){lo, hi}, bf16x2);
+    return __builtin_bit_cast(unsigned, p);
+}
+__device__ __forceinline__ float lo_bf16(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float hi_bf16(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+template <int G>
+__device__ __forceinline__ void st_group(bf16* p, const float (&v)[G]) {
+    if (G == 8) {
+        *reinterpret_cast<u32x4*>(p) = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[G - 4], v[G - 3]),
+                                             pack_bf16(v[G - 2], v[G - 1])};
+    } else {
+        *reinterpret_cast<u32x2*>(p) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    }
+}
+template <int G>
+__device__ __forceinline__ void ld_group(const bf16* p, float (&v)[G]) {
+    if (G == 8) {
+        const u32x4 u = *reinterpret_cast<const u32x4_a2*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[(2 * i) % G] = lo_bf16(u[i]), v[(2 * i + 1) % G] = hi_bf16(u[i]);
+    } else {
+        const u32x2 u = *reinterpret_cast<const u32x2_a2*>(p);
+        v[0] = lo_bf16(u[0]), v[1] = hi_bf16(u[0]), v[2] = lo_bf16(u[1]), v[3] = hi_bf16(u[1]);
+    }
+}
+
+// G neighbouring columns n .. n+G-1 (n a multiple of G) of row m; b: their bias.
+template <int G>
+__device__ __forceinline__ void finish_bf16(const Epilogue& p, int m, int n, float (&v)[G], const float (&b)[G]) {
+    if (m >= p.M || n >= p.n_pad) return;
+    const long long o = (long long)m * p.ldo + n;
+    const bool whole = n + G <= p.N;
+    float r[G];
+    if (p.res) {
+        const bf16* src = p.res + (long long)m * p.ldr + n;
+        if (whole) ld_group<G>(src, r);
+        else {
+#pragma unroll
+            for (int e = 0; e < G; ++e) r[e] = n + e < p.N ? (float)src[e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < G; ++e) v[e] += b[e];
+    if (!whole) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) v[e] = n + e < p.N ? v[e] : 0.0f;
+    }
+    const bool wide = p.vec && n + G <= p.n_pad;
+    if (p.z) {
+        if (wide) st_group<G>(p.z + o, v);
+        else {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+                if (n + e < p.n_pad) p.z[o + e] = (bf16)v[e];
+        }
+    }
+    if (p.act != LIN_NONE) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) v[e] = act_value(v[e], p.act);
+    }
+    if (p.res) {
+#pragma unroll
+        for (int e = 0; e < G; ++e) v[e] += r[e];
+    }
+    bf16* out = static_cast<bf16*>(p.out) + o;
+    if (wide) st_group<G>(out, v);
+    else {
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+            if (n + e < p.n_pad) out[e] = (bf16)v[e];
+    }
+}
+template <int G>
+__device__ __forceinline__ void finish_add(const Epilogue& p, int m, int n, const float (&v)[G]) {
+    if (m >= p.M) return;
+    float* out = static_cast<float*>(p.out) + (long long)m * p.ldo + n;
+#pragma unroll
+    for (int e = 0; e < G; ++e)
+        if (n + e < p.N) out[e] += v[e];                       // one writer per element
+}
+template <int G>
+__device__ __forceinline__ void ld_bias(const Epilogue& p, int n, float (&b)[G]) {
+#pragma unroll
+    for (int e = 0; e < G; ++e) b[e] = p.bias && n + e < p.N ? p.bias[n + e] : 0.0f;
+}
+
+// ------------------------------------------------------------------------------------------ tile kernel
+struct GemmParams {
+    const bf16* a;
+    const bf16* b;
+    unsigned long long a_bytes, b_bytes;
+    int lda, ldb, K;                   // K: reduction length, a multiple of 8 where an operand is K-contiguous
+    int splits, steps;                 // K ranges and 64-wide steps of one range
+    int tiles_m, tiles_n;
+    Epilogue ep;
+};
+
+#define LIN_BK 64
+
+__device__ __forceinline__ void lin_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds_wave_base, unsigned voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lin_lds_void_t*)lds_wave_base, 16, (int)voff, 0, 0, 0);
+}
+__device__ __forceinline__ bf16x8 lin_tr_pair(const unsigned char* lo, const unsigned char* hi) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    union { struct { s16x4 a, b; } s; bf16x8 v; } u;
+    u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)lo);
+    u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)hi);
+    return u.v;
+}
+
+// One operand of the tile: how its DMA is addressed and its fragments are read.  TR: K-strided.  R: rows (columns of the
+// memory image if TR) of the tile, NW: waves of the workgroup, PERM: fragment rows permuted (below).
+//
+// K-contiguous image: [R][64] bf16, 128-byte rows; LDS chunk c (16 bytes) of row r holds chunk c ^ key, key = (r >> 1) & 7,
+// so that the 16 rows of a fragment read fall on different banks.
+// K-strided image: [64][R], 2R-byte rows; a transposing read takes 4 k-rows x 16 columns per 16 lanes, and 32 lanes (rows
+// {0-3, 8-11} or {4-7, 12-15} of a 16-row group) are served at once: chunk c of row r holds chunk c ^ 2 key with
+// key = (r & 3) | (r >> 1 & 4), which puts those 8 rows on different banks.
+// PERM: which row of the operand an MFMA row stands for is free.  Row 16 (x >> 2) + 4 j + (x & 3) for row x of block j leaves
+// a lane with 16 neighbouring columns of the result, i.e. with whole 16-byte stores; the key then follows x.
+template <bool TR, int R, int NW, bool PERM>
+struct Operand {
+    static constexpr int BYTES = R * LIN_BK * 2, PER = BYTES / 1024 / NW;
+    static_assert(PER >= 1, "every wave takes part in staging");
+    static_assert(!(TR && PERM), "the permutation would put a transposing read's rows on the same banks");
+    unsigned voff[PER];
+    unsigned long long ptr;
+    long long left;
+    unsigned step;
+
+    static __device__ __forceinline__ int key(int row) {
+        if (PERM) row = ((row >> 4) & 3) * 4 + (row & 3);
+        return (row >> 1) & 7;
+    }
+    __device__ __forceinline__ static int dma_row(int wave, int lane, int j) {
+        return TR ? (wave * PER + j) * (512 / R) + lane / (R / 8) : (wave * PER + j) * 8 + (lane >> 3);
+    }
+    __device__ __forceinline__ static int dma_chunk(int lane, int row) {
+        return TR ? (lane % (R / 8)) ^ (2 * ((row & 3) | (row >> 1 & 4))) : (lane & 7) ^ key(row);
+    }
+    __device__ __forceinline__ void init(const bf16* x, unsigned long long bytes, int ld, int row0, int k0, int wave, int lane) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int row = dma_row(wave, lane, j);
+            voff[j] = (unsigned)row * (unsigned)ld * 2u + (unsigned)dma_chunk(lane, row) * 16u;
+        }
+        const unsigned long long off = TR ? ((unsigned long long)k0 * (unsigned)ld + (unsigned)row0) * 2ull
+                                          : ((unsigned long long)row0 * (unsigned)ld + (unsigned)k0) * 2ull;
+        ptr = (unsigned long long)x + off;
+        left = (long long)bytes - (long long)off;
+        step = TR ? (unsigned)(LIN_BK * 2) * (unsigned)ld : LIN_BK * 2u;
+    }
+    // stage the next 64 of K; `rem`: what is left of K from here (a K-contiguous row goes on behind it: those chunks are
+    // taken as zeros; a K-strided operand ends there, and the range check returns zeros)
+    __device__ __forceinline__ void issue(unsigned char* lds, int rem, int wave, int lane) {
+        const __amdgpu_buffer_rsrc_t rsrc =
+            make_rsrc(reinterpret_cast<const void*>(ptr), left <= 0 ? 0u : (left < 0x7fff0000ll ? (unsigned)left : 0x7fff0000u));
+        if (TR || rem >= LIN_BK) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) lin_dma16(rsrc, lds + (wave * PER + j) * 1024, voff[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                lin_dma16(rsrc, lds + (wave * PER + j) * 1024,
+                          dma_chunk(lane, dma_row(wave, lane, j)) * 8 < rem ? voff[j] : PDT_OOB_OFFSET);
+        }
+        ptr += step;
+        left -= step;
+    }
+    // fragment of 16 rows (block f of the wave's rows, which start at row0) and 32 k (half kk)
+    __device__ __forceinline__ static bf16x8 read(const unsigned char* lds, int row0, int f, int kk, int lane) {
+        if (TR) {
+            const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
+            const int r = kk * 32 + 8 * g + q, k2 = 2 * (q | (g & 1) * 4);
+            const int chunk = ((row0 + f * 16) / 8 + (pp >> 1)) ^ k2;
+            const unsigned char* at = lds + r * (R * 2) + chunk * 16 + (pp & 1) * 8;
+            return lin_tr_pair(at, at + 4 * (R * 2));
+        }
+        const int x = lane & 15;
+        const int row = row0 + (PERM ? 16 * (x >> 2) + 4 * f + (x & 3) : f * 16 + x);
+        return *reinterpret_cast<const bf16x8*>(lds + row * 128 + (((kk * 4 + (lane >> 4)) ^ key(row)) << 4));
+    }
+};
+
+template <int BM, int BN, int WM, int WN, bool AT, bool BT>
+__global__ __launch_bounds__(WM* WN * 64) void linear_gemm_kernel(const GemmParams p) {
+    constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
+    constexpr bool PERM = !BT && NI == 4;
+    typedef Operand<AT, BM, NW, false> A;
+    typedef Operand<BT, BN, NW, PERM> B;
+    constexpr int STAGE = A::BYTES + B::BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // ids 8 apart run on one XCD: each XCD gets a contiguous range of tiles, and tiles follow each other down columns of
+    // GROUP rows, so what runs at a time on an XCD is about square and shares its panels in that XCD's L2
+    constexpr int GROUP = 8;
+    int m0, n0, split;
+    {
+        const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
+        const int xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
+        int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+        split = id / per;
+        id -= split * per;
+        const int g = id / (GROUP * p.tiles_n), rows = min(GROUP, p.tiles_m - g * GROUP);
+        id -= g * GROUP * p.tiles_n;
+        m0 = (g * GROUP + id % rows) * BM;
+        n0 = id / rows * BN;
+    }
+    const int k0 = split * p.steps * LIN_BK;
+    const int nk = min(p.steps, (p.K - k0 + LIN_BK - 1) / LIN_BK);   // at least 1 (launcher)
+
+    A a;
+    B b;
+    a.init(p.a, p.a_bytes, p.lda, m0, k0, wave, lane);
+    b.init(p.b, p.b_bytes, p.ldb, n0, k0, wave, lane);
+
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    int rem = p.K - k0;
+    a.issue(smem, rem, wave, lane);
+    b.issue(smem + A::BYTES, rem, wave, lane);
+    for (int ks = 0; ks < nk; ++ks) {
+        unsigned char* cur = smem + (ks & 1) * STAGE;
+        unsigned char* nxt = smem + ((ks + 1) & 1) * STAGE;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's share of the stage has landed ...
+        __builtin_amdgcn_s_barrier();                          // ... every wave's has, and the other stage has been read
+        rem -= LIN_BK;
+        if (ks + 1 < nk) {
+            a.issue(nxt, rem, wave, lane);
+            b.issue(nxt + A::BYTES, rem, wave, lane);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            bf16x8 af[MI], bfr[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) bfr[j] = B::read(cur + A::BYTES, wn * WTN, j, kk, lane);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) af[i] = A::read(cur, wm * WTM, i, kk, lane);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[j], af[i], acc[i][j], 0, 0, 0);
+        }
+    }
+
+    // lane l holds row l & 15 of block i and, of block j, columns 4 (l >> 4) .. + 3 (PERM: 16 (l >> 4) + 4 j .. + 3)
+    const Epilogue& ep = p.ep;
+    const int fq = lane >> 4, mr = m0 + wm * WTM + (lane & 15), nb = n0 + wn * WTN;
+    if (ep.mode == OUT_BF16) {
+        if constexpr (PERM) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = nb + 16 * fq + 8 * h;
+                float bias[8];
+                ld_bias<8>(ep, n, bias);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = acc[i][2 * h + (e >> 2)][e & 3];
+                    finish_bf16<8>(ep, mr + i * 16, n, v, bias);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int n = nb + 16 * j + 4 * fq;
+                float bias[4];
+                ld_bias<4>(ep, n, bias);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+                    finish_bf16<4>(ep, mr + i * 16, n, v, bias);
+                }
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        const int n = nb + (PERM ? 16 * fq + 4 * j : 16 * j + 4 * fq);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+            if (ep.mode == OUT_ADD) finish_add<4>(ep, mr + i * 16, n, v);
+            else if (mr + i * 16 < ep.M) {
+                float* slab = ep.ws + ((long long)split * ep.M + mr + i * 16) * ep.N + n;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < ep.N) slab[e] = v[e];
+            }
+        }
+    }
+}
+
+// Joins the partial sums of a product whose K range was split (too few tiles for the chip), in slab order, and does what the
+// tile kernel's epilogue does.  mode: that of the result.
+__global__ __launch_bounds__(256) void linear_join_kernel(const Epilogue p, int splits) {
+    const int groups = (p.n_pad + 3) / 4;                      // (n_pad: N where the result has no padding)
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int m = (int)(t / groups), n = (int)(t % groups) * 4;
+    if (m >= p.M) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float* slab = p.ws + ((long long)s * p.M + m) * p.N + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < p.N) v[e] += slab[e];
+    }
+    if (p.mode == OUT_ADD) finish_add<4>(p, m, n, v);
+    else {
+        float bias[4];
+        ld_bias<4>(p, n, bias);
+        finish_bf16<4>(p, m, n, v, bias);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ few rows
+// Up to 16 * MT rows of a: bound by reading w once.  A wave takes 16 rows of w and a share of K and multiplies them with all
+// rows of a on the matrix cores, operands straight from memory (every element of w is used by one wave only, so LDS would
+// add nothing); the waves' sums meet in LDS.  Rows may start anywhere: unaligned 16-byte loads.
+template <int MT, int NW>
+__global__ __launch_bounds__(NW * 64) void linear_rows_kernel(const bf16* __restrict__ a, const bf16* __restrict__ w,
+                                                              long long lda, long long ldw, int K, const Epilogue ep) {
+    __shared__ f32x4 part[NW][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int x = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+    const bf16* wr = w + (long long)min(n0 + x, ep.N - 1) * ldw;       // rows past the end: computed and dropped
+    const bf16* ar[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) ar[t] = a + (long long)min(t * 16 + x, ep.M - 1) * lda;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const bf16* p, int k) -> bf16x8 { return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a2*>(p + k)); };
+    constexpr int U = 4;                                               // fragments of w a wave has in flight
+    const int steps = K / 32;
+    for (int r = wave * U; r < steps; r += NW * U) {
+        bf16x8 wf[U], af[MT][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = min(r + u, steps - 1) * 32 + g * 8;          // past the last step: loaded again, not multiplied
+            wf[u] = load(wr, k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) af[t][u] = load(ar[t], k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u < steps) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[u], af[t][u], acc[t], 0, 0, 0);
+            }
+    }
+    if (wave == NW - 1 && steps * 32 < K) {                            // the last, partial step
+        const int k = steps * 32 + g * 8;
+        auto load_part = [&](const bf16* p) -> bf16x8 {
+            if (k + 8 <= K) return load(p, k);
+            bf16x8 f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = k + e < K ? p[k + e] : (bf16)0.0f;
+            return f;
+        };
+        const bf16x8 wf = load_part(wr);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, load_part(ar[t]), acc[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < MT; t += NW) {
+        f32x4 s = part[0][t][lane];
+#pragma unroll
+        for (int v = 1; v < NW; ++v) s += part[v][t][lane];
+        float v[4] = {s[0], s[1], s[2], s[3]}, bias[4];
+        const int n = n0 + 4 * g;
+        ld_bias<4>(ep, n, bias);
+        finish_bf16<4>(ep, t * 16 + x, n, v, bias);
+    }
+    // columns of the padding that no 16-column block covers
+    const int done = gridDim.x * 16;
+    if (blockIdx.x == gridDim.x - 1)
+        for (int i = threadIdx.x; i < ep.M * (ep.n_pad - done); i += NW * 64) {
+            const long long o = (long long)(i / (ep.n_pad - done)) * ep.ldo + done + i % (ep.n_pad - done);
+            static_cast<bf16*>(ep.out)[o] = (bf16)0.0f;
+            if (ep.z) ep.z[o] = (bf16)0.0f;
+        }
+}
+
+// ------------------------------------------------------------------------------------------ backward of the activation
+// dz = dy * act'(z) in bf16 (rows padded with zeros to ldz columns: it is the next products' operand) and the column sums of
+// the unrounded dz, rows_per rows per block; partial sums of several row blocks are joined in order.
+// act == none: only the sums (dz == null) or also a padded copy of dy.
+__global__ __launch_bounds__(256) void linear_dz_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ z,
+                                                        bf16* __restrict__ dz, float* __restrict__ sums, long long ldy,
+                                                        long long ldzin, int ldz, int M, int N, int act, int rows_per, int add) {
+    __shared__ float red[8][32][8];
+    const int cv = threadIdx.x & 31, rr = threadIdx.x >> 5;
+    const int n = (blockIdx.x * 32 + cv) * 8;
+    const int r0 = blockIdx.y * rows_per, r1 = min(r0 + rows_per, M);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const bool whole = n + 8 <= N;
+    for (int m = r0 + rr; m < r1; m += 8) {
+        float g[8], x[8];
+        const bf16* src = dy + (long long)m * ldy + n;
+        const bf16* zs = z ? z + (long long)m * ldzin + n : nullptr;
+        if (whole) {
+            ld_group<8>(src, g);
+            if (zs) ld_group<8>(zs, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                g[e] = n + e < N ? (float)src[e] : 0.0f;
+                x[e] = zs && n + e < N ? (float)zs[e] : 0.0f;
+            }
+        }
+        if (zs) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = n + e < N ? g[e] * act_slope(x[e], act) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += g[e];
+        if (dz && n < ldz) st_group<8>(dz + (long long)m * ldz + n, g);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[rr][cv][e] = s[e];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= N) return;
+    float t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x >> 3][threadIdx.x & 7];
+    float* out = sums + (long long)blockIdx.y * N + c;
+    *out = add ? *out + t : t;
+}
+__global__ __launch_bounds__(256) void linear_sums_kernel(const float* __restrict__ part, float* __restrict__ out, int N,
+                                                          int parts, int add) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= N) return;
+    float t = 0.0f;
+    for (int i = 0; i < parts; ++i) t += part[(long long)i * N + c];
+    out[c] = add ? out[c] + t : t;
+}
+
+// rows of any stride and alignment -> rows of ldp columns (a multiple of 8), zeros behind the last one
+__global__ __launch_bounds__(256) void linear_pack_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst, long long ld,
+                                                          int ldp, int rows, int cols) {
+    const int vecs = ldp / 8;
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long row = t / vecs;
+    const int c = (int)(t % vecs) * 8;
+    if (row >= rows) return;
+    const bf16* s = src + row * ld + c;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (c + 8 <= cols) v = *reinterpret_cast<const u32x4_a2*>(s);
+    else {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = c + e < cols ? (float)s[e] : 0.0f;
+        v = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+    }
+    *reinterpret_cast<u32x4*>(dst + row * ldp + c) = v;
+}
+
+// ------------------------------------------------------------------------------------------ launchers
+#define LIN_MAX_LD (1 << 22)           // 256 rows of an operand stay below 2 GiB of 32-bit offsets
+#define LIN_CUS 256
+
+struct Plan {
+    int big, splits, steps, tiles_m, tiles_n;
+};
+static Plan plan_of(long long M, long long N, long long K) {
+    Plan q;
+    const int nk = cdiv(K, LIN_BK);
+    q.big = (long long)cdiv(M, 256) * cdiv(N, 256) >= LIN_CUS * 3 / 4;
+    const int t = q.big ? 256 : 128;
+    q.tiles_m = cdiv(M, t), q.tiles_n = cdiv(N, t);
+    const long long tiles = (long long)q.tiles_m * q.tiles_n;
+    q.splits = 1;
+    if (!q.big) {
+        while (tiles * q.splits * 2 <= 2 * LIN_CUS && nk / (q.splits * 2) >= 4) q.splits *= 2;
+    }
+    q.steps = cdiv(nk, q.splits);
+    q.splits = cdiv(nk, q.steps);
+    return q;
+}
+
+// floats of workspace that a product needs
+PDT_API long long pdt_linear_workspace(long long M, long long N, long long K) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const Plan q = plan_of(M, N, K);
+    return q.splits > 1 ? q.splits * M * N : 0;
+}
+
+static bool aligned16(const void* p) { return ((unsigned long long)p & 15) == 0; }
+
+template <bool AT, bool BT>
+static int launch_gemm(const bf16* a, const bf16* b, unsigned long long a_bytes, unsigned long long b_bytes, long long lda,
+                       long long ldb, int K, Epilogue ep, float* ws, hipStream_t s) {
+    if (!aligned16(a) || !aligned16(b) || lda % 8 || ldb % 8 || lda >= LIN_MAX_LD || ldb >= LIN_MAX_LD) return -2;
+    if ((!AT || !BT) && K % 8) return -2;
+    const Plan q = plan_of(ep.M, ep.N, K);
+    if ((long long)q.tiles_m * q.tiles_n * q.splits > 0x7fffffffll) return -1;
+    GemmParams p;
+    p.a = a, p.b = b, p.a_bytes = a_bytes, p.b_bytes = b_bytes, p.lda = (int)lda, p.ldb = (int)ldb, p.K = K;
+    p.splits = q.splits, p.steps = q.steps, p.tiles_m = q.tiles_m, p.tiles_n = q.tiles_n;
+    const int mode = ep.mode;
+    p.ep = ep;
+    if (q.splits > 1) {
+        if (!ws) return -3;
+        p.ep.mode = OUT_PART, p.ep.ws = ws;
+    }
+    const dim3 grid(q.tiles_m * q.tiles_n * q.splits);
+    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 2, 4, AT, BT>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, AT, BT>), grid, dim3(256), 0, s, p);
+    if (q.splits > 1) {
+        p.ep.mode = mode;
+        hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((ep.n_pad + 3) / 4) * ep.M, 256)), dim3(256), 0, s, p.ep, q.splits);
+    }
+    return pdt_launch_status();
+}
+
+static Epilogue plain_epilogue(void* out, int mode, int M, int N, long long ldo) {
+    Epilogue e;
+    e.out = out, e.z = nullptr, e.bias = nullptr, e.res = nullptr, e.ws = nullptr, e.ldr = 0;
+    e.ldo = (int)ldo, e.n_pad = N, e.M = M, e.N = N, e.mode = mode, e.act = LIN_NONE;
+    e.vec = ldo % 8 == 0 && aligned16(out);
+    return e;
+}
+static int pad8(int n) { return (n + 7) / 8 * 8; }
+// Memory of an operand: its rows hold a multiple of 8 columns (zeros behind the last one).  A descriptor that ended inside a
+// 4-byte word would return that word's valid half as zero too.
+static unsigned long long span_bytes(long long rows, int cols, long long ld) {
+    return ((unsigned long long)(rows - 1) * (unsigned long long)ld + (unsigned long long)pad8(cols)) * 2ull;
+}
+
+// Status -1: sizes, -2: alignment, -3: a workspace is needed.  The tile kernel's operands have rows that start at 16-byte
+// boundaries and are padded to a multiple of 8 columns, with zeros.
+// few: take the kernel for few rows (M <= 64), which needs no alignment.
+PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const void* res, void* y, void* z, void* ws, int M, int N,
+                           int K, long long lda, long long ldw, long long ldr, int ldo, int act, int few, hipStream_t s) {
+    if (M < 0 || N < 1 || K < 1 || ldo < N || ldo % 64 || act < 0 || act > LIN_SILU || (few && M > 64)) return -1;
+    if (M == 0) return 0;
+    Epilogue e = plain_epilogue(y, OUT_BF16, M, N, ldo);
+    e.z = static_cast<bf16*>(z), e.bias = static_cast<const float*>(bias), e.res = static_cast<const bf16*>(res);
+    e.ldr = ldr, e.act = act, e.n_pad = (N + 63) / 64 * 64;
+    const bf16 *ap = static_cast<const bf16*>(a), *wp = static_cast<const bf16*>(w);
+    if (few) {
+        const dim3 grid(cdiv(N, 16));
+        if (M <= 16) hipLaunchKernelGGL((linear_rows_kernel<1, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
+        else if (M <= 32) hipLaunchKernelGGL((linear_rows_kernel<2, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
+        else hipLaunchKernelGGL((linear_rows_kernel<4, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
+        return pdt_launch_status();
+    }
+    if (lda < pad8(K) || ldw < pad8(K)) return -2;
+    return launch_gemm<false, false>(ap, wp, span_bytes(M, K, lda), span_bytes(N, K, ldw), lda, ldw, K, e, static_cast<float*>(ws), s);
+}
+
+// da[M][K] = dz[M][N] w[N][K]
+PDT_API int pdt_linear_da(const void* dz, const void* w, void* da, void* ws, int M, int N, int K, long long lddz, long long ldw,
+                          long long ldda, hipStream_t s) {
+    if (M < 0 || N < 1 || K < 1 || ldda < K) return -1;
+    if (M == 0) return 0;
+    if (lddz < pad8(N) || ldw < pad8(K)) return -2;
+    return launch_gemm<false, true>(static_cast<const bf16*>(dz), static_cast<const bf16*>(w), span_bytes(M, N, lddz),
+                                    span_bytes(N, K, ldw), lddz, ldw, pad8(N), plain_epilogue(da, OUT_BF16, M, K, ldda),
+                                    static_cast<float*>(ws), s);
+}
+
+// dw[N][K] (bf16, or fp32 added to) = dz[M][N]^T a[M][K]
+PDT_API int pdt_linear_dw(const void* dz, const void* a, void* dw, void* ws, int M, int N, int K, long long lddz, long long lda,
+                          long long lddw, int add, hipStream_t s) {
+    if (M < 1 || N < 1 || K < 1 || lddw < K) return -1;
+    if (lddz < pad8(N) || lda < pad8(K)) return -2;
+    return launch_gemm<true, true>(static_cast<const bf16*>(dz), static_cast<const bf16*>(a), span_bytes(M, N, lddz),
+                                   span_bytes(M, K, lda), lddz, lda, M, plain_epilogue(dw, add ? OUT_ADD : OUT_BF16, N, K, lddw),
+                                   static_cast<float*>(ws), s);
+}
+
+// dz = dy act'(z) (dz may be null when act is none) and dbias (+)= its column sums; parts: row blocks, ws: parts * N floats
+// when parts > 1.
+PDT_API int pdt_linear_dz(const void* dy, const void* z, void* dz, void* dbias, void* ws, int M, int N, long long ldy, long long ldz,
+                          int lddz, int act, int parts, int add, hipStream_t s) {
+    if (M < 1 || N < 1 || act < 0 || act > LIN_SILU || parts < 1 || parts > 65535 || (act != LIN_NONE && (!z || !dz))) return -1;
+    if (dz && (lddz < pad8(N) || lddz % 8 || !aligned16(dz))) return -2;
+    if (parts > 1 && !ws) return -3;
+    const int cols = dz ? lddz : N;
+    float* out = static_cast<float*>(parts > 1 ? ws : dbias);
+    hipLaunchKernelGGL(linear_dz_kernel, dim3(cdiv(cols, 256), parts), dim3(256), 0, s, static_cast<const bf16*>(dy),
+                       act == LIN_NONE ? nullptr : static_cast<const bf16*>(z), static_cast<bf16*>(dz), out, ldy, ldz, lddz, M, N,
+                       act, cdiv(M, parts), parts > 1 ? 0 : add);
+    if (parts > 1)
+        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 256)), dim3(256), 0, s, out, static_cast<float*>(dbias), N, parts, add);
+    return pdt_launch_status();
+}
+
+PDT_API int pdt_linear_pack(const void* src, void* dst, long long ld, int ldp, int rows, int cols, hipStream_t s) {
+    if (rows < 0 || cols < 1 || ldp % 8 || ldp < cols || !aligned16(dst)) return -1;
+    if (rows == 0) return 0;
+    hipLaunchKernelGGL(linear_pack_kernel, dim3(cdiv((long long)rows * (ldp / 8), 256)), dim3(256), 0, s,
+                       static_cast<const bf16*>(src), static_cast<bf16*>(dst), ld, ldp, rows, cols);
+    return pdt_launch_status();
+}

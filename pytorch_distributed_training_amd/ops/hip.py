@@ -16,7 +16,7 @@ import torch
 
 from . import build as _build
 from .ref import MASK_NONE, MASK_RECOMPUTE, MASK_TENSOR  # noqa: F401  (re-exported)
-from .ref import check_distill_ce, check_top_logits
+from .ref import LINEAR_ACTS, check_distill_ce, check_linear_act_bwd, check_linear_act_fwd, check_top_logits
 
 name = "hip"
 # conv_dgrad reads the transposed copies ``wt`` only: the forward weights may be updated while backward still runs
@@ -99,6 +99,13 @@ _sig("pdt_bnfold_sums", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp)
 _sig("pdt_distill_ce", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _i, _i, _f, _f,
      _f, _vp)
 _sig("pdt_top_logits", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _f, _vp)
+_sig("pdt_linear_fwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i, _i, _vp)
+_sig("pdt_linear_da", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _vp)
+_sig("pdt_linear_dw", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _vp)
+_sig("pdt_linear_dz", _vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _i, _i, _i, _vp)
+_sig("pdt_linear_pack", _vp, _vp, _ll, _i, _i, _i, _vp)
+_sig("pdt_linear_workspace", _ll, _ll, _ll)
+_real.pdt_linear_workspace.restype = _ll
 _sig("pdt_set_deterministic", _i)
 _sig("pdt_accumulator_rows")
 
@@ -1266,6 +1273,80 @@ def ce_metrics(logits, labels):
     rc = _lib.pdt_ce_metrics(_p(logits), _p(labels.contiguous()), _p(out), B, N, logits.stride(0), _stream())
     _check(rc, "pdt_ce_metrics")
     return out
+
+
+# --------------------------------------------------------------------------- linear with activation and residual
+_FEW_ROWS = 32               # forward products of up to that many rows are bound by reading w once
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with rows that start and end at 16-byte boundaries (zeros behind the last column), as the tile kernel's staging
+    needs them: ``t`` itself, or a copy."""
+    rows, cols = t.shape
+    ld = t.stride(0)
+    if cols % 8 == 0 and ld % 8 == 0 and cols <= ld < 1 << 22 and t.data_ptr() % 16 == 0:
+        return t
+    out = torch.empty(rows, (cols + 7) // 8 * 8, dtype=t.dtype, device=t.device)
+    _check(_lib.pdt_linear_pack(t.data_ptr(), out.data_ptr(), ld, out.shape[1], rows, cols, _stream()), "pdt_linear_pack")
+    return out
+
+
+def _linear_workspace(M: int, N: int, K: int, device) -> Optional[torch.Tensor]:
+    floats = _real.pdt_linear_workspace(M, N, K)
+    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+
+
+def linear_act_fwd(a, w, bias=None, act: str = "none", residual=None, save: bool = False):
+    check_linear_act_fwd(a, w, bias, act, residual)
+    _here("linear_act_fwd", a, w, bias, residual)
+    M, K = a.shape
+    N, dev, ld = w.shape[0], a.device, _npad(w.shape[0])
+    y = torch.empty(M, ld, dtype=torch.bfloat16, device=dev)
+    z = torch.empty(M, ld, dtype=torch.bfloat16, device=dev) if save and act != "none" else None
+    few, ws = M <= _FEW_ROWS, None
+    if not few:
+        a, w = _rows16(a), _rows16(w)
+        K = (K + 7) // 8 * 8
+        ws = _linear_workspace(M, N, K, dev)
+    rc = _lib.pdt_linear_fwd(a.data_ptr(), w.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(z), _p(ws), M, N, K, a.stride(0),
+                             w.stride(0), residual.stride(0) if residual is not None else 0, ld, LINEAR_ACTS[act], int(few),
+                             _stream())
+    _check(rc, "pdt_linear_fwd")
+    return (y if ld == N else y[:, :N]), (z if z is None or ld == N else z[:, :N])
+
+
+def linear_act_bwd(a, w, dy, z=None, act: str = "none", dw=None, dbias=None, need_da: bool = True):
+    check_linear_act_bwd(a, w, dy, z, act, dw, dbias)
+    _here("linear_act_bwd", a, w, dy, z, dw, dbias)
+    M, K = a.shape
+    N, dev, st = w.shape[0], a.device, _stream()
+    da = torch.empty(M, K, dtype=torch.bfloat16, device=dev) if need_da else None
+    add_w, add_b = dw is not None, dbias is not None
+    if M == 0:
+        return (da, dw if add_w else torch.zeros(N, K, dtype=torch.bfloat16, device=dev),
+                dbias if add_b else torch.zeros(N, dtype=torch.float32, device=dev))
+    dw = dw if add_w else torch.empty(N, K, dtype=torch.bfloat16, device=dev)
+    dbias = dbias if add_b else torch.empty(N, dtype=torch.float32, device=dev)
+    # dy itself is the products' operand where there is no slope and its rows are aligned; else a padded bf16 dz
+    as_is = act == "none" and N % 8 == 0 and dy.stride(0) % 8 == 0 and N <= dy.stride(0) < 1 << 22 and dy.data_ptr() % 16 == 0
+    dz = dy if as_is else torch.empty(M, _npad(N), dtype=torch.bfloat16, device=dev)
+    # row blocks: about four workgroups per CU, each with at least 32 rows
+    parts = max(1, min((M + 31) // 32, 1024 * 256 // _npad(N)))
+    ws = torch.empty(parts * N, dtype=torch.float32, device=dev) if parts > 1 else None
+    rc = _lib.pdt_linear_dz(dy.data_ptr(), _p(z) if act != "none" else None, None if as_is else dz.data_ptr(), dbias.data_ptr(), _p(ws),
+                            M, N, dy.stride(0), z.stride(0) if z is not None else 0, dz.stride(0), LINEAR_ACTS[act], parts,
+                            int(add_b), st)
+    _check(rc, "pdt_linear_dz")
+    if need_da:
+        w16 = _rows16(w)
+        ws = _linear_workspace(M, K, (N + 7) // 8 * 8, dev)
+        _check(_lib.pdt_linear_da(dz.data_ptr(), w16.data_ptr(), da.data_ptr(), _p(ws), M, N, K, dz.stride(0), w16.stride(0), K, st),
+               "pdt_linear_da")
+    a16 = _rows16(a)
+    ws = _linear_workspace(N, K, M, dev)
+    _check(_lib.pdt_linear_dw(dz.data_ptr(), a16.data_ptr(), dw.data_ptr(), _p(ws), M, N, K, dz.stride(0), a16.stride(0),
+                              dw.stride(0), int(add_w), st), "pdt_linear_dw")
+    return da, dw, dbias
 
 
 # --------------------------------------------------------------------------- distillation

@@ -535,6 +535,121 @@ def ce_metrics(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     return torch.stack([loss_sum, (rank < 1).sum().float(), (rank < 5).sum().float(), n])
 
 
+# ---------------------------------------------------------------------------- linear with activation and residual
+LINEAR_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _check_rows(what: str, name: str, t: torch.Tensor, shape) -> None:
+    if t.dtype not in (torch.bfloat16, torch.float32) or (t.is_cuda and t.dtype != torch.bfloat16):
+        raise TypeError(f"{what}: {name} must be bf16 (the CPU path also takes fp32), got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: {name} must have unit column stride")
+
+
+def _check_vector(what: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} must be fp32, got {t.dtype}")
+    if tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: {name} must be contiguous [{n}], got {tuple(t.shape)}")
+
+
+def _check_product(what: str, a: torch.Tensor, w: torch.Tensor, act: str):
+    if act not in LINEAR_ACTS:
+        raise ValueError(f"{what}: act must be one of {sorted(LINEAR_ACTS)}, got {act!r}")
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1 or w.shape[0] < 1:
+        raise ValueError(f"{what}: a [M, K] and w [N, K] with K, N >= 1, got {tuple(a.shape)}, {tuple(w.shape)}")
+    _check_rows(what, "a", a, a.shape)
+    _check_rows(what, "w", w, w.shape)
+    return a.shape[0], w.shape[0], a.shape[1]
+
+
+def check_linear_act_fwd(a, w, bias, act: str, residual) -> None:
+    M, N, _ = _check_product("linear_act_fwd", a, w, act)
+    if bias is not None:
+        _check_vector("linear_act_fwd", "bias", bias, N)
+    if residual is not None:
+        _check_rows("linear_act_fwd", "residual", residual, (M, N))
+
+
+def check_linear_act_bwd(a, w, dy, z, act: str, dw, dbias) -> None:
+    what = "linear_act_bwd"
+    M, N, K = _check_product(what, a, w, act)
+    _check_rows(what, "dy", dy, (M, N))
+    if act != "none":
+        if z is None:
+            raise ValueError(f"{what}: act {act!r} needs z, the pre-activation that linear_act_fwd(save=True) returns")
+        _check_rows(what, "z", z, (M, N))
+    if dw is not None:
+        if dw.dtype != torch.float32:
+            raise TypeError(f"{what}: dw, where given, is a fp32 gradient buffer to add to, got {dw.dtype}")
+        if tuple(dw.shape) != (N, K) or (K > 1 and dw.stride(1) != 1) or (N > 1 and dw.stride(0) < K):
+            raise ValueError(f"{what}: dw must be [{N}, {K}] with unit column stride, got {tuple(dw.shape)}")
+    if dbias is not None:
+        _check_vector(what, "dbias", dbias, N)
+
+
+def _act_value(z: torch.Tensor, act: str) -> torch.Tensor:
+    if act == "relu":
+        return torch.relu(z)
+    if act == "gelu":
+        return torch.where(z == -torch.inf, torch.zeros_like(z), 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5))
+    if act == "silu":
+        return torch.where(z == -torch.inf, torch.zeros_like(z), z * torch.sigmoid(z))
+    return z
+
+
+def _act_slope(z: torch.Tensor, act: str) -> torch.Tensor:
+    if act == "relu":
+        return torch.where(z.isnan(), z, (z > 0).to(z.dtype))
+    big = z.isinf()
+    zf = torch.where(big, torch.zeros_like(z), z)
+    if act == "gelu":
+        slope = 0.5 * torch.special.erfc(-zf * 0.5 ** 0.5) + zf * torch.exp(-0.5 * zf * zf) * (0.5 / torch.pi) ** 0.5
+    else:
+        s = torch.sigmoid(zf)
+        slope = s * (1 + zf * (1 - s))
+    return torch.where(big, (z > 0).to(z.dtype), slope)
+
+
+def linear_act_fwd(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
+                   residual: Optional[torch.Tensor] = None, save: bool = False):
+    """``(y, z)``: ``z = a w^T + bias``, ``y = act(z) + residual``, each rounded once from fp32; ``a[M, K]``, ``w[N, K]``,
+    ``residual[M, N]`` in the compute dtype with unit column stride and any row stride, ``bias[N]`` fp32.
+
+    ``act``: none, relu, gelu (the exact one) or silu.  ``z`` is returned with ``save`` (what :func:`linear_act_bwd` needs where
+    there is an activation) and is None without it or with act none.  On the GPU ``y`` and ``z`` are views of rows padded to a
+    multiple of 64 columns, as :func:`linear_fwd` returns them, the padding zero."""
+    check_linear_act_fwd(a, w, bias, act, residual)
+    z = a.float() @ w.float().t()
+    if bias is not None:
+        z = z + bias
+    y = _act_value(z, act)
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(a.dtype), (z.to(a.dtype) if save and act != "none" else None)
+
+
+def linear_act_bwd(a: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, z: Optional[torch.Tensor] = None, act: str = "none",
+                   dw: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None, need_da: bool = True):
+    """Gradients ``(da, dw, dbias)`` of :func:`linear_act_fwd` for the gradient ``dy`` of its ``y`` (the residual's gradient is
+    ``dy`` itself): ``dz = dy act'(z)``, ``da = dz w``, ``dw = dz^T a``, ``dbias = sum of dz over the rows``.
+
+    ``dw`` / ``dbias`` given: fp32 gradient buffers, added to.  Not given: new tensors, ``dw`` in the compute dtype, ``dbias``
+    fp32.  ``need_da=False`` (a first layer): ``da`` is None.  On the GPU ``dz`` is rounded to bf16 before the products, as their
+    operand; ``dbias`` sums it unrounded.  Sums run in a fixed order: the same bits from run to run."""
+    check_linear_act_bwd(a, w, dy, z, act, dw, dbias)
+    dz = dy.float()
+    if act != "none":
+        dz = dz * _act_slope(z.float(), act)
+    da = (dz @ w.float()).to(a.dtype) if need_da else None
+    gw, gb = dz.t() @ a.float(), dz.sum(0)
+    dw = gw.to(a.dtype) if dw is None else dw.add_(gw)
+    dbias = gb if dbias is None else dbias.add_(gb)
+    return da, dw, dbias
+
+
 # ---------------------------------------------------------------------------- distillation
 MAX_TOP = 512                # slots per row
 MAX_CLASSES = 262144

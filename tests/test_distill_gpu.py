@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import _distill_oracle as oracle
+from pytorch_distributed_training_amd.engine.graphs import ListProgram
 from pytorch_distributed_training_amd.ops import ref
 
 pytestmark = pytest.mark.gpu
@@ -262,11 +263,12 @@ def test_captured_and_recorded(hip, device):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         captured = step()
-    items = []
-    hip.begin_recording(items)
-    recorded = step()
-    hip.end_recording()
-    assert len(items) == 2
+    program = ListProgram(device, hip)
+    with torch.cuda.use_mem_pool(program.pool):
+        program.begin()
+        recorded = step()
+        program.finish()
+    assert program.num_calls == 2
     for seed in range(4):
         gen = torch.Generator(device=device).manual_seed(seed)
         student.copy_(torch.randn(50, 3000, device=device, generator=gen))
@@ -276,6 +278,5 @@ def test_captured_and_recorded(hip, device):
         torch.cuda.synchronize()
         assert torch.equal(captured[0], want[0]) and torch.equal(captured[1], want[1])
         recorded[1].zero_()
-        for fn, args in items:
-            assert fn(*args) == 0
+        program.replay()
         assert torch.equal(recorded[0], want[0]) and torch.equal(recorded[1], want[1])
