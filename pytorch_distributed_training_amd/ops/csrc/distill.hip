@@ -125,8 +125,8 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Keeps the packed vector, not its fp32 values, in registers between two passes over a row, and one vector's work from
-// being interleaved with the next one's: both would double the registers of a wide row and spill it.
+// Ends one vector's share of a pass: the next pass unpacks the packed vector anew instead of keeping its fp32 values, and no
+// vector's work is interleaved with the next one's: either would double the registers of a wide row and spill it.
 __device__ __forceinline__ void hold(u32x4& r) {
     asm volatile("" : "+v"(r));
     __builtin_amdgcn_sched_barrier(0);
@@ -141,44 +141,63 @@ __device__ __forceinline__ int anew(int x) {
 
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// (... which what was computed from it must not outlive unfinished: with the sums as operands they are complete here)
+#define HOLD_STAT(r, s) asm volatile("" : "+v"(r), "+v"((s).m), "+v"((s).st), "+v"((s).s1)); __builtin_amdgcn_sched_barrier(0)
+
+// How exp(z - m) of the hard term follows from exp((z - m) / T) of the soft one, e.  An exponential takes four issue slots of
+// the vector unit, and with two of them per element and pass a wide row is bound by that unit, not by memory: the powers
+// measured 4096 x 131072 in POWERS_US us instead of 612.
+enum { EXP_ONE = 0,       // T = 1, or no hard term: one exponential
+       EXP_TWO = 1,       // any T: a second one
+       EXP_SQUARE = 2,    // T = 2: e^2
+       EXP_FOURTH = 4 };  // T = 4: e^4
+template <int MODE>
+__device__ __forceinline__ float hard_exp(float e, float d) {
+    if (MODE == EXP_TWO) return exp2_fast(d * DS_LOG2E);
+    if (MODE == EXP_SQUARE) return e * e;
+    if (MODE == EXP_FOURTH) return (e * e) * (e * e);
+    return e;
+}
+
 // Running maximum with two sums of exponentials relative to it: st with factor kt = log2(e) / T, s1 with log2(e).
 struct Stat {
     float m, st, s1;
 };
-template <bool TWO>
+template <int MODE>
 __device__ __forceinline__ Stat merge(Stat a, Stat b, float kt) {
     Stat r;
     r.m = fmaxf(a.m, b.m);
-    const float base = finite_or_zero(r.m);
-    r.st = a.st * exp2_fast((a.m - base) * kt) + b.st * exp2_fast((b.m - base) * kt);
-    r.s1 = TWO ? a.s1 * exp2_fast((a.m - base) * DS_LOG2E) + b.s1 * exp2_fast((b.m - base) * DS_LOG2E) : r.st;
+    const float base = finite_or_zero(r.m), da = a.m - base, db = b.m - base;
+    const float ea = exp2_fast(da * kt), eb = exp2_fast(db * kt);
+    r.st = a.st * ea + b.st * eb;
+    r.s1 = MODE ? a.s1 * hard_exp<MODE>(ea, da) + b.s1 * hard_exp<MODE>(eb, db) : r.st;
     return r;
 }
-template <bool TWO>
+template <int MODE>
 __device__ __forceinline__ Stat wave_merge(Stat a, float kt) {
-    const float m = wave_max(a.m), base = finite_or_zero(m);
-    a.st = wave_sum(a.st * exp2_fast((a.m - base) * kt));
-    a.s1 = TWO ? wave_sum(a.s1 * exp2_fast((a.m - base) * DS_LOG2E)) : a.st;
+    const float m = wave_max(a.m), d = a.m - finite_or_zero(m), e = exp2_fast(d * kt);
+    a.st = wave_sum(a.st * e);
+    a.s1 = MODE ? wave_sum(a.s1 * hard_exp<MODE>(e, d)) : a.st;
     a.m = m;
     return a;
 }
-template <bool TWO, int E>
+template <int MODE, int E>
 __device__ __forceinline__ void accumulate(Stat& s, const float (&f)[E], float kt) {
     float vm = f[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) vm = fmaxf(vm, f[e]);
     const float m = fmaxf(s.m, vm), base = finite_or_zero(m);
-    const float d0 = s.m - base;
-    float st = s.st * exp2_fast(d0 * kt), s1 = TWO ? s.s1 * exp2_fast(d0 * DS_LOG2E) : 0.0f;
+    const float d0 = s.m - base, e0 = exp2_fast(d0 * kt);
+    float st = s.st * e0, s1 = MODE ? s.s1 * hard_exp<MODE>(e0, d0) : 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const float d = f[e] - base;
-        st += exp2_fast(d * kt);
-        if (TWO) s1 += exp2_fast(d * DS_LOG2E);
+        const float d = f[e] - base, x = exp2_fast(d * kt);
+        st += x;
+        if (MODE) s1 += hard_exp<MODE>(x, d);
     }
     s.m = m;
     s.st = st;
-    s.s1 = TWO ? s1 : st;
+    s.s1 = MODE ? s1 : st;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -196,6 +215,9 @@ __device__ __forceinline__ void accumulate(Stat& s, const float (&f)[E], float k
 // classes does not underflow it.  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
 // after a barrier wave 0 rewrites the listed classes and the label (k + 1 elements).
 // ------------------------------------------------------------------------------------------
+#define DS_HEAD 256                 // bytes of the waves' statistics at the head of the LDS that is not row
+typedef __attribute__((address_space(3))) void ds_lds_void_t;
+
 struct DistillParams {
     const void* logits;
     const void* labels;
@@ -210,16 +232,18 @@ struct DistillParams {
     float inv_t, w_soft_grad, w_hard_grad, w_soft_loss, w_hard_loss;
 };
 
-template <typename T, int THREADS, int VPT, bool TWO>
+template <typename T, int THREADS, int VPT, int VL, int MODE>
 __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p) {
     constexpr int E = Pack<T>::E, W = THREADS / 64;
+    // one array: next to a second one the compiler waits for the copies into LDS before it reads either
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ Stat part[W + 1];
-    __shared__ float slot_sum;                                     // sum of P, negative: the row has no slots
+    constexpr int HELD = VL * THREADS * 16;                        // the row's second part
+    Stat* part = reinterpret_cast<Stat*>(lds + HELD);              // [W + 1]
+    float* slot_sum = reinterpret_cast<float*>(part + W + 1);      // sum of P, negative: the row has no slots
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x, N = p.N, k = p.k;
     const int nv = (N + E - 1) / E;
-    unsigned* bits = reinterpret_cast<unsigned*>(lds);
+    unsigned* bits = reinterpret_cast<unsigned*>(lds + HELD + DS_HEAD);
     const int words = ((N + 127) / 128) * 4;                       // a whole number of 16-byte stores
     int* s_idx = reinterpret_cast<int*>(bits + words);
     float* s_p = reinterpret_cast<float*>(s_idx + k);
@@ -231,22 +255,27 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const bool rest = p.lse != nullptr;
 
     u32x4 r[VPT > 0 ? VPT : 1];
-    if (VPT > 0) {
+    auto load_row = [&]() {
+        if (VPT > 0) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
-    }
+            for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
+        }
+        if (VL > 0) {                                              // (rows of whole vectors: launcher)
+            const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(src, (unsigned)N * (unsigned)sizeof(T));
+#pragma unroll
+            for (int j = 0; j < VL; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ds_lds_void_t*)(lds + (j * W + wave) * 1024), 16,
+                                                         ((VPT + j) * THREADS + tid) * 16, 0, 0, 0);
+        }
+    };
+    auto held = [&](int j) { return *reinterpret_cast<const u32x4*>(lds + (j * THREADS + tid) * 16); };
 
+    // the slots (wave 0): classes, their bits, values
     int label = -1;
-    float z_label = 0.0f;
-    if (p.labels) {
-        const long long l = p.label_bytes == 8 ? static_cast<const long long*>(p.labels)[row]
-                                               : (long long)static_cast<const int*>(p.labels)[row];
-        label = l >= 0 && l < N ? (int)l : -1;
-    }
-    if (wave == 0) {
+    float z_label = 0.0f, z_first = -INFINITY, tmax = -INFINITY;
+    bool twice = false;
+    auto load_slots = [&]() {
         for (int i = lane; i < words / 4; i += 64) reinterpret_cast<u32x4*>(bits)[i] = u32x4{0, 0, 0, 0};
-        bool twice = false;
-        float tmax = -INFINITY;
         for (int s = lane; s < k; s += 64) {
             const long long oi = (long long)row * p.ld_idx + s * p.st_idx;
             const long long li = p.index_bytes == 8 ? static_cast<const long long*>(p.indices)[oi]
@@ -254,16 +283,30 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
             float t = ld_as_float(p.values, (long long)row * p.ld_val + s * p.st_val, p.value_type);
             const int i = li >= 0 && li < N && t != -INFINITY ? (int)li : -1;
             t = i >= 0 ? t * p.inv_t : -INFINITY;
-            if (i >= 0) twice |= (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
+            if (i >= 0) {
+                twice |= (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
+                if (s == lane) z_first = (float)src[i];            // (used after the pass over the row: nobody waits for it)
+            }
             s_idx[s] = i;
             s_p[s] = t;
-            s_z[s] = i >= 0 ? (float)src[i] : -INFINITY;
-            tmax = t != t ? t : fmaxf(tmax, t);
+            tmax = t != t || tmax != tmax ? t + tmax : fmaxf(tmax, t);
         }
         if (label >= 0) z_label = (float)src[label];
+    };
+    if (p.labels) {
+        const long long l = p.label_bytes == 8 ? static_cast<const long long*>(p.labels)[row]
+                                               : (long long)static_cast<const int*>(p.labels)[row];
+        label = l >= 0 && l < N ? (int)l : -1;
+    }
+    // loads return in order: the slots come first where the other waves wait for them and the row is long
+    if (W > 1 && wave == 0) load_slots();
+    load_row();
+    if (W == 1) load_slots();
+    if (rest) lds_barrier();                                       // the bits are complete
+    if (wave == 0) {
         __builtin_amdgcn_wave_barrier();
-        const float top = wave_max(tmax);
         const bool any = __ballot(tmax != -INFINITY) != 0;         // a NaN counts: it shall reach the loss
+        const float top = wave_max(tmax);
         float total = 0.0f;
         for (int s = lane; s < k; s += 64) {
             const float t = s_p[s];
@@ -296,28 +339,23 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
                 s_p[s] = s_q[s] == -1.0f ? 0.0f : s_q[s];
             }
         }
-        Stat own = {-INFINITY, 0.0f, 0.0f};
-        if (rest)                                                  // the rest's sums skip the listed classes: theirs come from here
-            for (int s = lane; s < k; s += 64) {
-                const float f[1] = {s_idx[s] >= 0 ? s_z[s] : -INFINITY};
-                accumulate<TWO, 1>(own, f, kt);
-            }
-        own = wave_merge<TWO>(own, kt);
-        if (lane == 0) {
-            part[W] = own;
-            slot_sum = any ? total : -1.0f;
-        }
+        if (lane == 0) *slot_sum = any ? total : -1.0f;
     }
-    if (rest) lds_barrier();                                       // the bits are complete
 
     Stat mine = {-INFINITY, 0.0f, 0.0f};
     // -inf for what this vector repeats of an earlier one and, with a rest, for the listed classes
     auto take_out = [&](u32x4 q, int v, bool whole) -> u32x4 {
         if (!whole) q = drop_repeated<T>(q, v, N);
         if (rest) {
-            const int c = first_class<T>(v, N);
-            unsigned b = bits[c >> 5] >> (c & 31);
-            if ((c & 31) > 32 - E) b |= bits[(c >> 5) + 1] << (32 - (c & 31));
+            unsigned b;
+            if (whole) {                                           // starts at a multiple of E: within one byte
+                const unsigned c = (unsigned)v * E;
+                b = reinterpret_cast<const unsigned char*>(bits)[c >> 3] >> (c & 7);
+            } else {
+                const int c = first_class<T>(v, N);
+                b = bits[c >> 5] >> (c & 31);
+                if ((c & 31) > 32 - E) b |= bits[(c >> 5) + 1] << (32 - (c & 31));
+            }
             b &= (1u << E) - 1u;
             if (b) {
                 float f[E];
@@ -336,8 +374,20 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
             r[j] = take_out(r[j], j * THREADS + t, (j + 1) * THREADS * E <= N);
             float f[E];
             Pack<T>::unpack(r[j], f);
-            accumulate<TWO, E>(mine, f, kt);
-            hold(r[j]);
+            accumulate<MODE, E>(mine, f, kt);
+            HOLD_STAT(r[j], mine);
+        }
+        if (VL > 0) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // what this wave copied into LDS is there: nobody else reads it
+            for (int j = 0; j < VL; ++j) {
+                const int v = (VPT + j) * THREADS + tid;
+                if (v >= nv) break;
+                const u32x4 q = take_out(held(j), v, true);
+                if (rest) *reinterpret_cast<u32x4*>(lds + (j * THREADS + tid) * 16) = q;
+                float f[E];
+                Pack<T>::unpack(q, f);
+                accumulate<MODE, E>(mine, f, kt);
+            }
         }
     } else {
         for (int v = tid; v < nv; v += 4 * THREADS) {
@@ -349,22 +399,34 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
             for (int u = 0; u < 4; ++u) {
                 float f[E];
                 Pack<T>::unpack(take_out(q[u], v + u * THREADS, whole), f);
-                accumulate<TWO, E>(mine, f, kt);
+                accumulate<MODE, E>(mine, f, kt);
             }
         }
     }
-    mine = wave_merge<TWO>(mine, kt);
+    if (wave == 0) {                                               // the listed classes' own logits and, with a rest, sums
+        Stat own = {-INFINITY, 0.0f, 0.0f};
+        for (int s = lane; s < k; s += 64) {
+            const int i = s_idx[s];
+            const float z = s == lane ? z_first : i >= 0 ? (float)src[i] : -INFINITY;
+            s_z[s] = z;
+            const float f[1] = {i >= 0 ? z : -INFINITY};
+            if (rest) accumulate<MODE, 1>(own, f, kt);
+        }
+        own = wave_merge<MODE>(own, kt);
+        if (lane == 0) part[W] = own;
+    }
+    mine = wave_merge<MODE>(mine, kt);
     if (lane == 0) part[wave] = mine;
     lds_barrier();
 
     // every wave works out the row's numbers for itself
     Stat a = part[0];
 #pragma unroll
-    for (int w = 1; w < W; ++w) a = merge<TWO>(a, part[w], kt);
-    const Stat all = rest ? merge<TWO>(a, part[W], kt) : a;
+    for (int w = 1; w < W; ++w) a = merge<MODE>(a, part[w], kt);
+    const Stat all = rest ? merge<MODE>(a, part[W], kt) : a;
     const float m = all.m;
     const bool some = m != -INFINITY || all.st != all.st;          // a row of -inf has no distribution: it counts for nothing
-    const float sum_p = slot_sum;
+    const float sum_p = *slot_sum;
     const bool soft = some && !(sum_p < 0.0f);
     const float base = finite_or_zero(a.m);
     const float inv_st = some ? 1.0f / all.st : 0.0f, inv_s1 = some ? 1.0f / all.s1 : 0.0f;
@@ -384,8 +446,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
         Pack<T>::unpack(q, f);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = f[e] - base;
-            g[e] = TWO ? ct * exp2_fast(d * kt) + c1 * exp2_fast(d * DS_LOG2E) : cs * exp2_fast(d * kt);
+            const float d = f[e] - base, x = exp2_fast(d * kt);
+            if (MODE == EXP_TWO) g[e] = ct * x + c1 * exp2_fast(d * DS_LOG2E);
+            else if (MODE == EXP_SQUARE) g[e] = x * (ct + c1 * x);
+            else if (MODE == EXP_FOURTH) g[e] = x * (ct + (c1 * x) * (x * x));
+            else g[e] = cs * x;
         }
         if (whole || (v + 1) * E <= N) {
             __builtin_nontemporal_store(Pack<T>::pack(g),
@@ -403,6 +468,11 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
         for (int j = 0; j < VPT; ++j) {
             gradient(r[j], j * THREADS + t, (j + 1) * THREADS * E <= N);
             hold(r[j]);
+        }
+        for (int j = 0; j < VL; ++j) {
+            const int v = (VPT + j) * THREADS + tid;
+            if (v >= nv) break;
+            gradient(held(j), v, true);
         }
     } else {
         for (int v = tid; v < nv; v += 4 * THREADS) {
@@ -462,20 +532,35 @@ __global__ __launch_bounds__(256) void distill_mean_kernel(const float* __restri
     if (threadIdx.x == 0) *out = n > 0 ? (float)(red[0] / (double)n) : 0.0f;
 }
 
-template <typename T, bool TWO>
+template <typename T, int MODE>
 static void launch_distill(const DistillParams& p, hipStream_t s) {
-    const int nv = (p.N + Pack<T>::E - 1) / Pack<T>::E;
-    const size_t shared = (size_t)((p.N + 127) / 128) * 16 + (size_t)p.k * 16;
+    constexpr int NARROW = MODE == EXP_ONE ? EXP_ONE : EXP_TWO;    // (those are bound by latency, not by exponentials)
+    constexpr int E = Pack<T>::E;
+    const int nv = (p.N + E - 1) / E;
+    const size_t shared = DS_HEAD + (size_t)((p.N + 127) / 128) * 16 + (size_t)p.k * 16;
     const dim3 grid(p.B);
-#define DS_LAUNCH(TH, V) hipLaunchKernelGGL((distill_kernel<T, TH, V, TWO>), grid, dim3(TH), shared, s, p)
-    if (nv <= 64) DS_LAUNCH(64, 1);
-    else if (nv <= 128) DS_LAUNCH(64, 2);
-    else if (nv <= 256) DS_LAUNCH(64, 4);
-    else if (nv <= 1024) DS_LAUNCH(256, 4);
-    else if (nv <= 4096) DS_LAUNCH(1024, 4);
-    else if (nv <= 8192) DS_LAUNCH(1024, 8);
-    else DS_LAUNCH(1024, 0);
+    // rows that start and end at 16-byte boundaries may be copied into LDS
+    const bool whole = p.N % E == 0 && p.ld_in % E == 0 && ((unsigned long long)p.logits & 15) == 0;
+#define DS_LAUNCH(TH, V, L, MD) \
+    hipLaunchKernelGGL((distill_kernel<T, TH, V, L, MD>), grid, dim3(TH), shared + (size_t)L * TH * 16, s, p)
+    if (nv <= 64) DS_LAUNCH(64, 1, 0, NARROW);
+    else if (nv <= 128) DS_LAUNCH(64, 2, 0, NARROW);
+    else if (nv <= 256) DS_LAUNCH(64, 4, 0, NARROW);
+    else if (nv <= 1024) DS_LAUNCH(256, 4, 0, NARROW);
+    else if (nv <= 4096) DS_LAUNCH(1024, 4, 0, MODE);
+    else if (nv <= 8192 && whole) DS_LAUNCH(1024, 4, 4, MODE);
+    else if (nv <= 8192) DS_LAUNCH(1024, 8, 0, MODE);
+    else if (nv <= 16384 && whole) DS_LAUNCH(1024, 8, 8, MODE);
+    else DS_LAUNCH(1024, 0, 0, MODE);
 #undef DS_LAUNCH
+}
+
+template <typename T>
+static void launch_distill(const DistillParams& p, int mode, hipStream_t s) {
+    if (mode == EXP_ONE) launch_distill<T, EXP_ONE>(p, s);
+    else if (mode == EXP_SQUARE) launch_distill<T, EXP_SQUARE>(p, s);
+    else if (mode == EXP_FOURTH) launch_distill<T, EXP_FOURTH>(p, s);
+    else launch_distill<T, EXP_TWO>(p, s);
 }
 
 // Status -1: an argument outside what the kernel is built for (nothing was launched).
@@ -500,10 +585,13 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
         p.w_hard_loss = labels ? 1.0f - alpha : 0.0f;
         p.w_soft_grad = alpha * temperature * grad_scale / (float)B;
         p.w_hard_grad = p.w_hard_loss * grad_scale / (float)B;
-        const bool two = p.w_hard_loss != 0.0f && temperature != 1.0f;
-        if (type == DS_BF16) two ? launch_distill<bf16, true>(p, s) : launch_distill<bf16, false>(p, s);
-        else if (type == DS_FP16) two ? launch_distill<f16, true>(p, s) : launch_distill<f16, false>(p, s);
-        else two ? launch_distill<float, true>(p, s) : launch_distill<float, false>(p, s);
+        const int mode = p.w_hard_loss == 0.0f || temperature == 1.0f ? EXP_ONE
+                         : temperature == 2.0f                        ? EXP_SQUARE
+                         : temperature == 4.0f                        ? EXP_FOURTH
+                                                                      : EXP_TWO;
+        if (type == DS_BF16) launch_distill<bf16>(p, mode, s);
+        else if (type == DS_FP16) launch_distill<f16>(p, mode, s);
+        else launch_distill<float>(p, mode, s);
         const int rc = pdt_launch_status();
         if (rc != 0) return rc;
     }
@@ -518,9 +606,10 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
 // A lower bound of the k-th largest comes from the threads' own maxima: with W waves, the smallest over the waves of the
 // ceil(k / W)-th largest lane maximum has at least k elements at or above it, and for values in no particular order only
 // a few times k.  Those candidates go to LDS as 64-bit keys (value, then class) and are sorted there; the keys differ, so
-// the order in which the candidates arrive does not matter.  Rows on which the bound is too low (many equal values,
-// sorted rows) are cut to exactly k candidates by bisecting the value and, among equals, the class: exact, some 50
-// passes over the registers.
+// the order in which the candidates arrive does not matter.  The bound is taken from the row's first chunk, which waits for it
+// in registers, and again whenever twice as much has been read; the rest of the row streams past it: the row is read once.
+// Rows on which the bound is too low (many equal values, sorted rows) or that hold a NaN or +inf are cut to exactly k
+// candidates by bisecting the value and, among equals, the class: exact, some 50 more passes over the row.
 // ------------------------------------------------------------------------------------------
 struct TopParams {
     const void* logits;
@@ -548,10 +637,10 @@ __device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v,
 
 template <typename T, int THREADS, int VPT>
 __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) {
-    constexpr int E = Pack<T>::E, W = THREADS / 64, CAP = THREADS == 64 ? 512 : 2048;
+    constexpr int E = Pack<T>::E, W = THREADS / 64, CAP = THREADS == 64 ? 512 : THREADS == 256 ? 2048 : 4096;
     __shared__ unsigned long long cand[CAP];
     __shared__ Stat part[W];
-    __shared__ float bound[W];
+    __shared__ float bound[2][W];
     __shared__ int tally[W];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -559,88 +648,116 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
     const int nv = (N + E - 1) / E;
     const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld_in;
     const float kt = p.inv_t * DS_LOG2E;
+    if (tid == 0) count = 0;                                       // (a barrier follows before the first use)
 
-    u32x4 r[VPT > 0 ? VPT : 1];
-    if (VPT > 0) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
-    }
-    if (VPT > 0) {
-        const int t = anew(tid);
-#pragma unroll
-        for (int j = 0; j < VPT; ++j)
-            if ((j + 1) * THREADS * E > N) r[j] = drop_repeated<T>(r[j], j * THREADS + t, N);
-    }
-    auto over_row = [&](auto&& fn) {                               // fn(values, first class) for every vector of this thread
-        if (VPT > 0) {
-            const int t = anew(tid);
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                float f[E];
-                Pack<T>::unpack(r[j], f);
-                fn(f, first_class<T>(j * THREADS + t, N));
-                hold(r[j]);
-            }
-        } else {
-            for (int v = tid; v < nv; v += 4 * THREADS) {
-                u32x4 q[4];
-                const bool whole = (long long)(v - tid + 4 * THREADS) * E <= N;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) q[u] = ld_row<T, false>(src, v + u * THREADS, N);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float f[E];
-                    Pack<T>::unpack(whole ? q[u] : drop_repeated<T>(q[u], v + u * THREADS, N), f);
-                    fn(f, first_class<T>(v + u * THREADS, N));
-                }
-            }
-        }
-    };
     auto keep = [&](float f, int c) {
         const int at = atomicAdd(&count, 1);
         if (at < CAP) cand[at] = slot_key(f, c);
     };
-
     Stat mine = {-INFINITY, 0.0f, 0.0f};
-    over_row([&](const float (&f)[E], int) { accumulate<false, E>(mine, f, kt); });
-    float v = mine.m;                                              // sorted over the wave, falling
+    int turn = 0;
+    float floor_v = -INFINITY;
+    const int rank = (k + W - 1) / W;                              // at most 64 (launcher)
+    auto raise_floor = [&]() {                                     // (all threads)
+        // the 16 leading bits of the rank-th largest maximum of the wave: bisected with ballots
+        const unsigned key = order_key(mine.m);
+        unsigned t = 0;
 #pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            const float o = __shfl_xor(v, step, 64);
-            v = ((lane & step) == 0) == ((lane & size) == 0) ? fmaxf(v, o) : fminf(v, o);
+        for (int b = 31; b >= 16; --b) {
+            const unsigned c = t | 1u << b;
+            if (__popcll(__ballot(key >= c)) >= rank) t = c;
         }
-    const float low = __shfl(v, (k + W - 1) / W - 1, 64);
-    mine = wave_merge<false>(mine, kt);
-    if (lane == 0) {
-        bound[wave] = low;
-        part[wave] = mine;
-    }
-    if (tid == 0) count = 0;
-    lds_barrier();
-    float floor_v = bound[0];
+        if (lane == 0) bound[turn][wave] = t <= 0x007fffffu ? -INFINITY : __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
+        lds_barrier();
+        float f = bound[turn][0];
 #pragma unroll
-    for (int w = 1; w < W; ++w) floor_v = fminf(floor_v, bound[w]);
-    if (tid == 0) {
-        Stat a = part[0];
-        for (int w = 1; w < W; ++w) a = merge<false>(a, part[w], kt);
-        p.lse[row] = finite_or_zero(a.m) * p.inv_t + logf(a.st);
-    }
-    over_row([&](const float (&f)[E], int c) {
-        bool any = false;
+        for (int w = 1; w < W; ++w) f = fminf(f, bound[turn][w]);
+        floor_v = f;
+        turn ^= 1;                                                 // the next round writes the other set: one barrier each
+    };
+    auto collect = [&](const float (&f)[E], int v) {
+        float m = f[0];
 #pragma unroll
-        for (int e = 0; e < E; ++e) any |= !(f[e] < floor_v);      // NaN too
-        if (any) {
+        for (int e = 1; e < E; ++e) m = fmaxf(m, f[e]);
+        if (m >= floor_v) {
+            const int c = first_class<T>(v, N);
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (!(f[e] < floor_v) && f[e] != -INFINITY) keep(f[e], c + e);
+                if (f[e] >= floor_v && f[e] != -INFINITY) keep(f[e], c + e);
         }
-    });
+    };
+    {
+        u32x4 r[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) r[j] = ld_row<T, VPT == 1>(src, j * THREADS + tid, N);
+        int t = anew(tid);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            if ((j + 1) * THREADS * E > N) r[j] = drop_repeated<T>(r[j], j * THREADS + t, N);
+            float f[E];
+            Pack<T>::unpack(r[j], f);
+            accumulate<EXP_ONE, E>(mine, f, kt);
+            HOLD_STAT(r[j], mine);
+        }
+        raise_floor();
+        t = anew(tid);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            float f[E];
+            Pack<T>::unpack(r[j], f);
+            collect(f, j * THREADS + t);
+            hold(r[j]);
+        }
+    }
+    // the rest, two vectors at a time with the next two on their way
+    constexpr int U = 2;
+    if (nv > VPT * THREADS) {
+        u32x4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = ld_row<T, false>(src, VPT * THREADS + u * THREADS + tid, N);
+        int raise_at = 2 * VPT * THREADS;                          // vectors read when the floor is raised next
+        for (int v0 = VPT * THREADS; v0 < nv; v0 += U * THREADS) {
+            u32x4 nx[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) nx[u] = ld_row<T, false>(src, v0 + (U + u) * THREADS + tid, N);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int v = v0 + u * THREADS + tid;
+                if ((v0 + (u + 1) * THREADS) * E > N) q[u] = drop_repeated<T>(q[u], v, N);
+                float f[E];
+                Pack<T>::unpack(q[u], f);
+                accumulate<EXP_ONE, E>(mine, f, kt);
+                collect(f, v);
+                HOLD_STAT(nx[u], mine);
+                q[u] = nx[u];
+            }
+            if (v0 + U * THREADS == raise_at && raise_at < nv) {
+                raise_floor();
+                raise_at *= 2;
+            }
+        }
+    }
+    mine = wave_merge<EXP_ONE>(mine, kt);
+    if (lane == 0) part[wave] = mine;
     lds_barrier();
+    if (tid == 0) {
+        Stat a = part[0];
+        for (int w = 1; w < W; ++w) a = merge<EXP_ONE>(a, part[w], kt);
+        p.lse[row] = finite_or_zero(a.m) * p.inv_t + logf(a.st);
+    }
     int n = count;
+    bool plain = true;                                             // no NaN, no +inf: those make the sum NaN
+#pragma unroll
+    for (int w = 0; w < W; ++w) plain &= part[w].st == part[w].st;
 
-    if (n > CAP) {                                                 // the bound was too low for this row
+    auto over_row = [&](auto&& fn) {                               // fn(values, first class) for every vector of this thread
+        for (int v = tid; v < nv; v += THREADS) {
+            float f[E];
+            Pack<T>::unpack(drop_repeated<T>(ld_row<T, true>(src, v, N), v, N), f);
+            fn(f, first_class<T>(v, N));
+        }
+    };
+    if (n > CAP || !plain) {
         auto total = [&](int mine_n) {
             const int t = (int)wave_sum((float)mine_n);            // below 2^24: exact
             lds_barrier();                                         // the last round's tallies have been read
@@ -651,7 +768,13 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
             for (int w = 0; w < W; ++w) s += tally[w];
             return s;
         };
-        unsigned t = 0;                                            // largest key that k elements reach
+        int filled = 0;
+        over_row([&](const float (&f)[E], int) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) filled += f[e] != -INFINITY;
+        });
+        const int want = min(k, total(filled));
+        unsigned t = 0;                                            // largest key that `want` elements reach
         for (int b = 31; b >= 0; --b) {
             const unsigned c = t | 1u << b;
             int m = 0;
@@ -659,14 +782,14 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
 #pragma unroll
                 for (int e = 0; e < E; ++e) m += f[e] != -INFINITY && order_key(f[e]) >= c;
             });
-            if (total(m) >= k) t = c;
+            if (total(m) >= want) t = c;
         }
         int above = 0;
         over_row([&](const float (&f)[E], int) {
 #pragma unroll
             for (int e = 0; e < E; ++e) above += f[e] != -INFINITY && order_key(f[e]) > t;
         });
-        const int need = k - total(above);
+        const int need = want - total(above);
         int lo = 0, hi = N - 1;                                    // smallest class up to which `need` elements equal the key
         while (lo < hi) {
             const int mid = lo + (hi - lo) / 2;
@@ -736,14 +859,14 @@ template <typename T>
 static void launch_top(const TopParams& p, int B, hipStream_t s) {
     const int nv = (p.N + Pack<T>::E - 1) / Pack<T>::E;
 #define DS_LAUNCH(TH, V) hipLaunchKernelGGL((top_logits_kernel<T, TH, V>), dim3(B), dim3(TH), 0, s, p)
-    // at least two threads per wanted logit: with fewer the bound from the thread maxima lets too many candidates pass
+    // at least two threads per wanted logit: with fewer the bound from the thread maxima lets too many candidates pass.
+    // Wide rows: small workgroups where there are rows for several on every CU (one's loads run under another's sort)
+    const bool many = B >= 4 * 256;
     if (nv <= 64 && p.k <= 32) DS_LAUNCH(64, 1);
     else if (nv <= 128 && p.k <= 32) DS_LAUNCH(64, 2);
     else if (nv <= 256 && p.k <= 32) DS_LAUNCH(64, 4);
-    else if (nv <= 1024 && p.k <= 128) DS_LAUNCH(256, 4);
-    else if (nv <= 4096) DS_LAUNCH(1024, 4);
-    else if (nv <= 8192) DS_LAUNCH(1024, 8);
-    else DS_LAUNCH(1024, 0);
+    else if ((nv <= 1024 || many) && p.k <= 128) DS_LAUNCH(256, 4);
+    else DS_LAUNCH(1024, 4);
 #undef DS_LAUNCH
 }
 

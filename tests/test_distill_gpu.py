@@ -52,6 +52,16 @@ def test_distill(hip, device, rows, classes, k, dtype, tail):
         check(hip, args, temperature, alpha, 64.0)
 
 
+@pytest.mark.parametrize("classes", [9000, 40000, 50001, 65536, 100000, 131072, 140000])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0, 4.0])
+def test_distill_both_terms_on_wide_rows(hip, device, classes, dtype, temperature):
+    """Every way to the hard term's exponentials, rows that are held in registers, in LDS too, and read twice."""
+    for wide, tail in ((0, True), (4, False)):
+        args = oracle.inputs(2, classes, 20, dtype, temperature, classes, True, tail, device, wide)
+        check(hip, args, temperature, 0.4, 16.0)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("classes", [30, 5000])
 def test_distill_slots(hip, device, tail, classes):
@@ -142,9 +152,9 @@ def test_more_than_four_gigabytes_of_logits(hip, device):
     block = torch.randn(100, classes, device=device).to(torch.bfloat16)
     logits.view(90, 100, classes).copy_(block)
     values, indices, lse = hip.top_logits(logits, k, 2.0)
-    want = hip.top_logits(logits[-3:].clone(), k, 2.0)
+    want = hip.top_logits(logits[-1100:].clone(), k, 2.0)         # (as many rows as take the same kernel)
     for a, b in zip((values, indices, lse), want):
-        assert torch.equal(a[-3:], b)
+        assert torch.equal(a[-1100:], b)
     labels = torch.arange(rows, device=device)
     _, grad = hip.distill_ce(logits, labels, values, indices, 2.0, 0.5, lse, float(rows))
     _, want = hip.distill_ce(logits[-3:].clone(), labels[-3:], values[-3:], indices[-3:], 2.0, 0.5, lse[-3:], 3.0)
@@ -196,6 +206,20 @@ def test_top_logits_of_rows_that_defeat_the_bound(hip, device, classes):
     for dtype in (torch.float32, torch.bfloat16):
         for k in (1, 31, 100, 500):
             check_top(hip, rows.to(dtype), k, 1.0)
+
+
+@pytest.mark.parametrize("k", [1, 64, 128, 300])
+def test_top_logits_of_many_wide_rows(hip, device, k):
+    """Enough rows for several workgroups per CU; rows that defeat the bound among them."""
+    gen = torch.Generator(device=device).manual_seed(k)
+    logits = torch.randn(1100, 20011, device=device, generator=gen).to(torch.bfloat16)
+    up = torch.arange(20011, device=device)
+    logits[3], logits[4], logits[5] = 1.0, up.to(torch.bfloat16), (-up).to(torch.bfloat16)
+    logits[6] = -math.inf
+    logits[7, 20000] = math.nan
+    logits[8, 11] = math.inf
+    logits[9, 40:] = -math.inf
+    check_top(hip, logits, k, 1.0)
 
 
 def test_refusals(hip, device):
