@@ -775,6 +775,8 @@ __global__ __launch_bounds__(256, 2) void conv_dma_kernel(const ConvDmaParams p)
             gy0 = rem / (unsigned)p.Wg;
             gx0 = rem - gy0 * (unsigned)p.Wg;
         }
+        // in vector registers: with the backward-sums operands next to them the scalar ones run out
+        if constexpr (BSTAT) asm volatile("" : "+v"(gb0), "+v"(gy0), "+v"(gx0));
         const size_t orow0 = (size_t)(any_live ? roww : p.M - 1);
 #pragma unroll
         for (int i0 = 0; i0 < MI; i0 += EG) {
