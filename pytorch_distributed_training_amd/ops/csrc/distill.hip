@@ -768,12 +768,13 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
             for (int w = 0; w < W; ++w) s += tally[w];
             return s;
         };
-        int filled = 0;
+        int filled = 0, nans = 0;
         over_row([&](const float (&f)[E], int) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) filled += f[e] != -INFINITY;
+            for (int e = 0; e < E; ++e) filled += f[e] != -INFINITY, nans += f[e] != f[e];
         });
         const int want = min(k, total(filled));
+        if (!plain && total(nans) == 0 && tid == 0) p.lse[row] = INFINITY;   // +inf and no NaN
         unsigned t = 0;                                            // largest key that `want` elements reach
         for (int b = 31; b >= 0; --b) {
             const unsigned c = t | 1u << b;
