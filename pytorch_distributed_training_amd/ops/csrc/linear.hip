@@ -9,6 +9,7 @@
 // (buffer_load ... lds, no staging registers) and differ in how fragments are read back: ds_read_b128 for the first,
 // the transposing ds_read_b64_tr_b16 for the second.  No operand is ever transposed in memory.
 #include "common.h"
+#include <type_traits>
 
 #define LIN_NONE 0
 #define LIN_RELU 1
@@ -155,15 +156,23 @@ template <int G>
 __device__ __forceinline__ void finish_add(const Epilogue& p, int m, int n, const float (&v)[G]) {
     if (m >= p.M) return;
     float* out = static_cast<float*>(p.out) + (long long)m * p.ldo + n;
+    if (p.vec && n + G <= p.N) {                               // one writer per element
+#pragma unroll
+        for (int e = 0; e < G; e += 4) *reinterpret_cast<f32x4*>(out + e) += f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < G; ++e)
-        if (n + e < p.N) out[e] += v[e];                       // one writer per element
+        if (n + e < p.N) out[e] += v[e];
 }
 template <int G>
 __device__ __forceinline__ void ld_bias(const Epilogue& p, int n, float (&b)[G]) {
 #pragma unroll
     for (int e = 0; e < G; ++e) b[e] = p.bias && n + e < p.N ? p.bias[n + e] : 0.0f;
 }
+
+// Partial sums: [splits][M][slab_ld(N)], rows of whole 8-column groups.
+__host__ __device__ __forceinline__ long long slab_ld(int N) { return (N + 7) / 8 * 8; }
 
 // ------------------------------------------------------------------------------------------ tile kernel
 struct GemmParams {
@@ -178,9 +187,6 @@ struct GemmParams {
 
 #define LIN_BK 64
 
-__device__ __forceinline__ void lin_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char* lds_wave_base, unsigned voff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lin_lds_void_t*)lds_wave_base, 16, (int)voff, 0, 0, 0);
-}
 __device__ __forceinline__ bf16x8 lin_tr_pair(const unsigned char* lo, const unsigned char* hi) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     union { struct { s16x4 a, b; } s; bf16x8 v; } u;
@@ -199,9 +205,9 @@ __device__ __forceinline__ bf16x8 lin_tr_pair(const unsigned char* lo, const uns
 // key = (r & 3) | (r >> 1 & 4), which puts those 8 rows on different banks.
 // PERM: which row of the operand an MFMA row stands for is free.  Row 16 (x >> 2) + 4 j + (x & 3) for row x of block j leaves
 // a lane with 16 neighbouring columns of the result, i.e. with whole 16-byte stores; the key then follows x.
-template <bool TR, int R, int NW, bool PERM>
+template <bool TR, int R, int NW, bool PERM, int BK>
 struct Operand {
-    static constexpr int BYTES = R * LIN_BK * 2, PER = BYTES / 1024 / NW;
+    static constexpr int BYTES = R * BK * 2, PER = BYTES / 1024 / NW, CH = BK / 8;   // CH: chunks of a K-contiguous row
     static_assert(PER >= 1, "every wave takes part in staging");
     static_assert(!(TR && PERM), "the permutation would put a transposing read's rows on the same banks");
     unsigned voff[PER];
@@ -211,13 +217,13 @@ struct Operand {
 
     static __device__ __forceinline__ int key(int row) {
         if (PERM) row = ((row >> 4) & 3) * 4 + (row & 3);
-        return (row >> 1) & 7;
+        return BK == 64 ? (row >> 1) & 7 : (row >> 1) & 2;
     }
     __device__ __forceinline__ static int dma_row(int wave, int lane, int j) {
-        return TR ? (wave * PER + j) * (512 / R) + lane / (R / 8) : (wave * PER + j) * 8 + (lane >> 3);
+        return TR ? (wave * PER + j) * (512 / R) + lane / (R / 8) : (wave * PER + j) * (64 / CH) + lane / CH;
     }
     __device__ __forceinline__ static int dma_chunk(int lane, int row) {
-        return TR ? (lane % (R / 8)) ^ (2 * ((row & 3) | (row >> 1 & 4))) : (lane & 7) ^ key(row);
+        return TR ? (lane % (R / 8)) ^ (2 * ((row & 3) | (row >> 1 & 4))) : (lane % CH) ^ key(row);
     }
     __device__ __forceinline__ void init(const bf16* x, unsigned long long bytes, int ld, int row0, int k0, int wave, int lane) {
 #pragma unroll
@@ -229,22 +235,23 @@ struct Operand {
                                           : ((unsigned long long)row0 * (unsigned)ld + (unsigned)k0) * 2ull;
         ptr = (unsigned long long)x + off;
         left = (long long)bytes - (long long)off;
-        step = TR ? (unsigned)(LIN_BK * 2) * (unsigned)ld : LIN_BK * 2u;
+        step = TR ? (unsigned)(BK * 2) * (unsigned)ld : BK * 2u;
     }
-    // stage the next 64 of K; `rem`: what is left of K from here (a K-contiguous row goes on behind it: those chunks are
-    // taken as zeros; a K-strided operand ends there, and the range check returns zeros)
-    __device__ __forceinline__ void issue(unsigned char* lds, int rem, int wave, int lane) {
-        const __amdgpu_buffer_rsrc_t rsrc =
-            make_rsrc(reinterpret_cast<const void*>(ptr), left <= 0 ? 0u : (left < 0x7fff0000ll ? (unsigned)left : 0x7fff0000u));
-        if (TR || rem >= LIN_BK) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) lin_dma16(rsrc, lds + (wave * PER + j) * 1024, voff[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                lin_dma16(rsrc, lds + (wave * PER + j) * 1024,
-                          dma_chunk(lane, dma_row(wave, lane, j)) * 8 < rem ? voff[j] : PDT_OOB_OFFSET);
-        }
+    __device__ __forceinline__ u32x4 desc() const {
+        const unsigned n = left <= 0 ? 0u : (left < 0x7fff0000ll ? (unsigned)left : 0x7fff0000u);
+        return u32x4{(unsigned)ptr, (unsigned)(ptr >> 32) & 0xffffu, n, 0x00020000u};
+    }
+    // piece j of this wave's share of a stage, to LDS offset m (moved on to the next piece's).  TAIL: `rem` may be less than a
+    // stage: a K-contiguous row goes on behind K, those chunks are taken as zeros (a K-strided operand ends there, and the
+    // range check returns zeros)
+    template <bool TAIL>
+    __device__ __forceinline__ void piece(u32x4 d, unsigned& m, int rem, int j, int wave, int lane) const {
+        unsigned v = voff[j];
+        if (TAIL && !TR) v = dma_chunk(lane, dma_row(wave, lane, j)) * 8 < rem ? v : PDT_OOB_OFFSET;
+        asm volatile("s_mov_b32 m0, %0\n\ts_add_u32 %0, %0, 0x400\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     : "+s"(m) : "v"(v), "s"(d) : "memory", "scc");
+    }
+    __device__ __forceinline__ void next() {
         ptr += step;
         left -= step;
     }
@@ -258,19 +265,19 @@ struct Operand {
             return lin_tr_pair(at, at + 4 * (R * 2));
         }
         const int x = lane & 15;
-        const int row = row0 + (PERM ? 16 * (x >> 2) + 4 * f + (x & 3) : f * 16 + x);
-        return *reinterpret_cast<const bf16x8*>(lds + row * 128 + (((kk * 4 + (lane >> 4)) ^ key(row)) << 4));
+        const int row = row0 + (PERM ? (f >> 2) * 64 + 16 * (x >> 2) + 4 * (f & 3) + (x & 3) : f * 16 + x);
+        return *reinterpret_cast<const bf16x8*>(lds + row * (BK * 2) + (((kk * 4 + (lane >> 4)) ^ key(row)) << 4));
     }
 };
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT>
-__global__ __launch_bounds__(WM* WN * 64) void linear_gemm_kernel(const GemmParams p) {
+template <int BM, int BN, int WM, int WN, int BK, int RING, bool AT, bool BT>
+__global__ __launch_bounds__(WM* WN * 64, BM == 256 || RING > 2 ? 1 : 2) void linear_gemm_kernel(const GemmParams p) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
-    constexpr bool PERM = !BT && NI == 4;
-    typedef Operand<AT, BM, NW, false> A;
-    typedef Operand<BT, BN, NW, PERM> B;
+    constexpr bool PERM = !BT && NI % 4 == 0;
+    typedef Operand<AT, BM, NW, false, BK> A;
+    typedef Operand<BT, BN, NW, PERM, BK> B;
     constexpr int STAGE = A::BYTES + B::BYTES;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[MI == 8 && NI == 8 ? 5 * A::BYTES : RING * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -290,7 +297,7 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_gemm_kernel(const GemmPara
         n0 = id / rows * BN;
     }
     const int k0 = split * p.steps * LIN_BK;
-    const int nk = min(p.steps, (p.K - k0 + LIN_BK - 1) / LIN_BK);   // at least 1 (launcher)
+    const int nk = (min(p.steps * LIN_BK, p.K - k0) + BK - 1) / BK;   // stages, at least 1 (launcher)
 
     A a;
     B b;
@@ -303,83 +310,169 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_gemm_kernel(const GemmPara
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    int rem = p.K - k0;
-    a.issue(smem, rem, wave, lane);
-    b.issue(smem + A::BYTES, rem, wave, lane);
-    for (int ks = 0; ks < nk; ++ks) {
-        unsigned char* cur = smem + (ks & 1) * STAGE;
-        unsigned char* nxt = smem + ((ks + 1) & 1) * STAGE;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's share of the stage has landed ...
-        __builtin_amdgcn_s_barrier();                          // ... every wave's has, and the other stage has been read
-        rem -= LIN_BK;
-        if (ks + 1 < nk) {
-            a.issue(nxt, rem, wave, lane);
-            b.issue(nxt + A::BYTES, rem, wave, lane);
+    int rem = p.K - k0;                                        // of K, from the stage that is staged next
+    constexpr int PIECES = A::PER + B::PER;
+    const unsigned lds0 = (unsigned)(unsigned long long)(lin_lds_void_t*)smem;
+    if constexpr (MI == 8 && NI == 8) {
+        bf16x8 a0[MI], b0[NI], a1[MI], b1[NI];
+        int rem_b = rem;
+        // slot of operand stage n (a: 2 ks, b: 2 ks + 1) is n mod 5
+        auto half = [&](const bf16x8 (&ac)[MI], const bf16x8 (&bc)[NI], bf16x8 (&an)[MI], bf16x8 (&bn)[NI], int sa, int sb, int kk,
+                        auto&& dma) {
+            const unsigned char *as = smem + sa * A::BYTES, *bs = smem + sb * A::BYTES;
+#pragma unroll
+            for (int g = 0; g < 16; ++g) {
+                if (g < 4) {
+                    bn[2 * g] = B::read(bs, wn * WTN, 2 * g, kk, lane);
+                    bn[2 * g + 1] = B::read(bs, wn * WTN, 2 * g + 1, kk, lane);
+                } else if (g < 8) {
+                    an[(2 * g - 8)&7] = A::read(as, wm * WTM, 2 * g - 8, kk, lane);
+                    an[(2 * g - 7)&7] = A::read(as, wm * WTM, 2 * g - 7, kk, lane);
+                }
+                if (g % 2 == 0) dma(g / 2);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int i = (4 * g + t) / NI, j = (4 * g + t) % NI;
+                    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(bc[j]), "v"(ac[i]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        const unsigned wave_at = lds0 + wave * (A::PER * 1024);
+        auto stage_a = [&](int slot) {
+            const u32x4 d = a.desc();
+            unsigned m = wave_at + slot * A::BYTES;
+#pragma unroll
+            for (int j = 0; j < A::PER; ++j) a.template piece<true>(d, m, rem, j, wave, lane);
+            a.next();
+            rem -= BK;
+        };
+        auto stage_b = [&](int slot) {
+            const u32x4 d = b.desc();
+            unsigned m = wave_at + slot * A::BYTES;
+#pragma unroll
+            for (int j = 0; j < B::PER; ++j) b.template piece<true>(d, m, rem_b, j, wave, lane);
+            b.next();
+            rem_b -= BK;
+        };
+        stage_a(0);
+        stage_b(1);
+        stage_a(2);
+        stage_b(3);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b0[j] = B::read(smem + A::BYTES, wn * WTN, j, 0, lane);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a0[i] = A::read(smem, wm * WTM, i, 0, lane);
+        int sa = 0;                                            // slot of a's stage ks
+        auto up = [](int s, int n) { return s + n >= 5 ? s + n - 5 : s + n; };
+        auto k_step = [&](auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
+            {
+                const u32x4 d = a.desc();
+                unsigned m = wave_at + up(sa, 4) * A::BYTES;
+                half(a0, b0, a1, b1, sa, up(sa, 1), 1, [&](int j) { a.template piece<TAIL>(d, m, rem, j, wave, lane); });
+                a.next();
+                rem -= BK;
+            }
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(A::PER) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            {
+                const u32x4 d = b.desc();
+                unsigned m = wave_at + sa * A::BYTES;
+                half(a1, b1, a0, b0, up(sa, 2), up(sa, 3), 0, [&](int j) { b.template piece<TAIL>(d, m, rem_b, j, wave, lane); });
+                b.next();
+                rem_b -= BK;
+            }
+            sa = up(sa, 2);
+        };
+        const int whole = min(rem / BK, nk);                   // steps that stage whole stages
+        int ks = 0;
+        for (; ks < whole; ++ks) k_step(std::integral_constant<bool, false>{});
+        for (; ks < nk; ++ks) k_step(std::integral_constant<bool, true>{});
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
+    } else {
+        bf16x8 af[MI], bfr[NI];
+        unsigned fill = 0, at = 0;                             // slots: staged next, read
+        auto stage = [&]() {
+            const u32x4 da = a.desc(), db = b.desc();
+            unsigned ma = lds0 + fill * STAGE + wave * (A::PER * 1024), mb = lds0 + fill * STAGE + A::BYTES + wave * (B::PER * 1024);
+#pragma unroll
+            for (int j = 0; j < A::PER; ++j) a.template piece<true>(da, ma, rem, j, wave, lane);
+#pragma unroll
+            for (int j = 0; j < B::PER; ++j) b.template piece<true>(db, mb, rem, j, wave, lane);
+            a.next();
+            b.next();
+            rem -= BK;
+            fill = fill == RING - 1 ? 0 : fill + 1;
+        };
+#pragma unroll
+        for (int s = 0; s < RING - 1; ++s) stage();            // (past the end of K: zeros)
+        for (int g = 0; g < nk; ++g) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * PIECES) : "memory");   // this wave's share has landed ...
+            __builtin_amdgcn_s_barrier();                      // ... every wave's has, and the stage before has been read
+            asm volatile("" ::: "memory");
+            stage();
+            const unsigned char* cur = smem + at * STAGE;
+#pragma unroll
+            for (int kk = 0; kk < BK / 32; ++kk) {
+#pragma unroll
+                for (int j = 0; j < NI; ++j) bfr[j] = B::read(cur + A::BYTES, wn * WTN, j, kk, lane);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) af[i] = A::read(cur, wm * WTM, i, kk, lane);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[j], af[i], acc[i][j], 0, 0, 0);
+            }
+            at = at == RING - 1 ? 0 : at + 1;
         }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf16x8 af[MI], bfr[NI];
-#pragma unroll
-            for (int j = 0; j < NI; ++j) bfr[j] = B::read(cur + A::BYTES, wn * WTN, j, kk, lane);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) af[i] = A::read(cur, wm * WTM, i, kk, lane);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[j], af[i], acc[i][j], 0, 0, 0);
-        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
-    // lane l holds row l & 15 of block i and, of block j, columns 4 (l >> 4) .. + 3 (PERM: 16 (l >> 4) + 4 j .. + 3)
+    // The sums go through LDS: a lane holds row x = l & 15 of block i and, of block j, four neighbouring columns; out of LDS a
+    // thread takes eight neighbouring columns of a row, so that whole rows are loaded (residual) and stored, and what is done to
+    // them is one short loop.  (Straight from the accumulators, unrolled over them, this took 98 000 cycles of a 256 x 256
+    // tile: as long as 40 K steps.)  16-byte chunk c of a row is kept at c ^ x: the 16 rows of a write fall on different banks.
     const Epilogue& ep = p.ep;
-    const int fq = lane >> 4, mr = m0 + wm * WTM + (lane & 15), nb = n0 + wn * WTN;
-    if (ep.mode == OUT_BF16) {
-        if constexpr (PERM) {
+    constexpr int PI = MI < 4 ? MI : 4, ROWS = WM * PI * 16, NT = NW * 64, COLS8 = BN / 8;
+    static_assert(ROWS * BN * 4 <= sizeof(smem), "a pass fits");
+    const int x = lane & 15, fq = lane >> 4;
+    const int n = n0 + (int)(threadIdx.x % COLS8) * 8;
+    float bias[8];
+    ld_bias<8>(ep, n, bias);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = nb + 16 * fq + 8 * h;
-                float bias[8];
-                ld_bias<8>(ep, n, bias);
+    for (int h = 0; h < MI / PI; ++h) {
+        __syncthreads();                                       // what was in LDS has been read (and every DMA has landed)
 #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[i][2 * h + (e >> 2)][e & 3];
-                    finish_bf16<8>(ep, mr + i * 16, n, v, bias);
-                }
-            }
-        } else {
+        for (int i = 0; i < PI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const int n = nb + 16 * j + 4 * fq;
-                float bias[4];
-                ld_bias<4>(ep, n, bias);
-#pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-                    finish_bf16<4>(ep, mr + i * 16, n, v, bias);
-                }
+                const int row = (wm * PI + i) * 16 + x;
+                const int chunk = (wn * WTN + (PERM ? (j >> 2) * 64 + 16 * fq + 4 * (j & 3) : 16 * j + 4 * fq)) / 4;
+                *reinterpret_cast<f32x4*>(smem + row * (BN * 4) + ((chunk ^ x) << 4)) = acc[h * PI + i][j];
             }
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-        const int n = nb + (PERM ? 16 * fq + 4 * j : 16 * j + 4 * fq);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-            if (ep.mode == OUT_ADD) finish_add<4>(ep, mr + i * 16, n, v);
-            else if (mr + i * 16 < ep.M) {
-                float* slab = ep.ws + ((long long)split * ep.M + mr + i * 16) * ep.N + n;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < ep.N) slab[e] = v[e];
+        __syncthreads();
+        for (int row = threadIdx.x / COLS8; row < ROWS; row += NT / COLS8) {
+            const int m = m0 + row / (PI * 16) * WTM + h * PI * 16 + row % (PI * 16);
+            const int chunk = (threadIdx.x % COLS8) * 2, key = row & 15;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((chunk ^ key) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + (((chunk + 1) ^ key) << 4));
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (ep.mode == OUT_BF16) finish_bf16<8>(ep, m, n, v, bias);
+            else if (ep.mode == OUT_ADD) finish_add<8>(ep, m, n, v);
+            else if (m < ep.M && n < ep.N) {
+                float* slab = ep.ws + ((long long)split * ep.M + m) * slab_ld(ep.N) + n;
+                *reinterpret_cast<f32x4*>(slab) = lo;
+                *reinterpret_cast<f32x4*>(slab + 4) = hi;
             }
         }
     }
@@ -388,22 +481,24 @@ __global__ __launch_bounds__(WM* WN * 64) void linear_gemm_kernel(const GemmPara
 // Joins the partial sums of a product whose K range was split (too few tiles for the chip), in slab order, and does what the
 // tile kernel's epilogue does.  mode: that of the result.
 __global__ __launch_bounds__(256) void linear_join_kernel(const Epilogue p, int splits) {
-    const int groups = (p.n_pad + 3) / 4;                      // (n_pad: N where the result has no padding)
+    const int groups = (p.n_pad + 7) / 8;                      // (n_pad: N where the result has no padding)
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int m = (int)(t / groups), n = (int)(t % groups) * 4;
+    const int m = (int)(t / groups), n = (int)(t % groups) * 8;
     if (m >= p.M) return;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-        const float* slab = p.ws + ((long long)s * p.M + m) * p.N + n;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < p.N) {
+        const float* slab = p.ws + m * slab_ld(p.N) + n;
+        for (int s = 0; s < splits; ++s, slab += p.M * slab_ld(p.N)) {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(slab), hi = *reinterpret_cast<const f32x4*>(slab + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) v[e] += slab[e];
+            for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
+        }
     }
-    if (p.mode == OUT_ADD) finish_add<4>(p, m, n, v);
+    if (p.mode == OUT_ADD) finish_add<8>(p, m, n, v);
     else {
-        float bias[4];
-        ld_bias<4>(p, n, bias);
-        finish_bf16<4>(p, m, n, v, bias);
+        float bias[8];
+        ld_bias<8>(p, n, bias);
+        finish_bf16<8>(p, m, n, v, bias);
     }
 }
 
@@ -568,9 +663,7 @@ static Plan plan_of(long long M, long long N, long long K) {
     q.tiles_m = cdiv(M, t), q.tiles_n = cdiv(N, t);
     const long long tiles = (long long)q.tiles_m * q.tiles_n;
     q.splits = 1;
-    if (!q.big) {
-        while (tiles * q.splits * 2 <= 2 * LIN_CUS && nk / (q.splits * 2) >= 4) q.splits *= 2;
-    }
+    if (!q.big && tiles < LIN_CUS) q.splits = (int)max(1ll, min(LIN_CUS / tiles, (long long)nk / 4));
     q.steps = cdiv(nk, q.splits);
     q.splits = cdiv(nk, q.steps);
     return q;
@@ -580,7 +673,7 @@ static Plan plan_of(long long M, long long N, long long K) {
 PDT_API long long pdt_linear_workspace(long long M, long long N, long long K) {
     if (M < 1 || N < 1 || K < 1) return 0;
     const Plan q = plan_of(M, N, K);
-    return q.splits > 1 ? q.splits * M * N : 0;
+    return q.splits > 1 ? q.splits * M * slab_ld((int)N) : 0;
 }
 
 static bool aligned16(const void* p) { return ((unsigned long long)p & 15) == 0; }
@@ -602,11 +695,12 @@ static int launch_gemm(const bf16* a, const bf16* b, unsigned long long a_bytes,
         p.ep.mode = OUT_PART, p.ep.ws = ws;
     }
     const dim3 grid(q.tiles_m * q.tiles_n * q.splits);
-    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 2, 4, AT, BT>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, AT, BT>), grid, dim3(256), 0, s, p);
+    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 2, 2, 64, 2, AT, BT>), grid, dim3(256), 0, s, p);
+    else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, 64, 4, AT, BT>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, 64, 2, AT, BT>), grid, dim3(256), 0, s, p);
     if (q.splits > 1) {
         p.ep.mode = mode;
-        hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((ep.n_pad + 3) / 4) * ep.M, 256)), dim3(256), 0, s, p.ep, q.splits);
+        hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((ep.n_pad + 7) / 8) * ep.M, 256)), dim3(256), 0, s, p.ep, q.splits);
     }
     return pdt_launch_status();
 }
