@@ -125,6 +125,29 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// Sum / maximum over a wave by DPP moves (a shuffle goes through LDS: at six of them per reduction and some ten reductions
+// per row they were half of a narrow row's time).  The same order every time; every lane gets the result.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_or(float identity, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(identity), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+template <typename Op>
+__device__ __forceinline__ float wave_reduce(float v, float identity, Op op) {
+    v = op(v, dpp_or<0x111, 0xf>(identity, v));                    // row_shr:1, 2, 4, 8 inside the rows of 16 lanes
+    v = op(v, dpp_or<0x112, 0xf>(identity, v));
+    v = op(v, dpp_or<0x114, 0xf>(identity, v));
+    v = op(v, dpp_or<0x118, 0xf>(identity, v));
+    v = op(v, dpp_or<0x142, 0xa>(identity, v));                    // row_bcast:15 into rows 1 and 3
+    v = op(v, dpp_or<0x143, 0xc>(identity, v));                    // row_bcast:31 into rows 2 and 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_top(float v) {
+    return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // Ends one vector's share of a pass: the next pass unpacks the packed vector anew instead of keeping its fp32 values, and no
 // vector's work is interleaved with the next one's: either would double the registers of a wide row and spill it.
 __device__ __forceinline__ void hold(u32x4& r) {
@@ -175,9 +198,9 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b, float kt) {
 }
 template <int MODE>
 __device__ __forceinline__ Stat wave_merge(Stat a, float kt) {
-    const float m = wave_max(a.m), d = a.m - finite_or_zero(m), e = exp2_fast(d * kt);
-    a.st = wave_sum(a.st * e);
-    a.s1 = MODE ? wave_sum(a.s1 * hard_exp<MODE>(e, d)) : a.st;
+    const float m = wave_top(a.m), d = a.m - finite_or_zero(m), e = exp2_fast(d * kt);
+    a.st = wave_total(a.st * e);
+    a.s1 = MODE ? wave_total(a.s1 * hard_exp<MODE>(e, d)) : a.st;
     a.m = m;
     return a;
 }
@@ -306,7 +329,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     if (wave == 0) {
         __builtin_amdgcn_wave_barrier();
         const bool any = __ballot(tmax != -INFINITY) != 0;         // a NaN counts: it shall reach the loss
-        const float top = wave_max(tmax);
+        const float top = wave_top(tmax);
         float total = 0.0f;
         for (int s = lane; s < k; s += 64) {
             const float t = s_p[s];
@@ -314,7 +337,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
             s_p[s] = e;
             total += e;
         }
-        total = wave_sum(total);
+        total = wave_total(total);
         if (!rest && any) {
             const float inv = 1.0f / total;
             for (int s = lane; s < k; s += 64) s_p[s] *= inv;
@@ -500,7 +523,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
         dst[i] = (T)g;
         label_listed |= i == label;
     }
-    loss = wave_sum(loss);
+    loss = wave_total(loss);
     label_listed = __ballot(label_listed) != 0;
     if (lane == 0) {
         if (soft && has_rest && p_rest > 0.0f)
@@ -759,7 +782,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
     };
     if (n > CAP || !plain) {
         auto total = [&](int mine_n) {
-            const int t = (int)wave_sum((float)mine_n);            // below 2^24: exact
+            const int t = (int)wave_total((float)mine_n);            // below 2^24: exact
             lds_barrier();                                         // the last round's tallies have been read
             if (lane == 0) tally[wave] = t;
             lds_barrier();
@@ -826,9 +849,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
     if (n <= 64) {                                                 // one wave, in registers
         if (wave != 0) return;
         unsigned long long key = lane < n ? cand[lane] : 0ull;
-#pragma unroll
-        for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
+        for (int size = 2; size < 2 * n; size <<= 1)               // (lanes past the next power of two keep their zeros)
             for (int step = size >> 1; step > 0; step >>= 1) {
                 const unsigned long long o = shfl_xor_u64(key, step);
                 const bool take_max = ((lane & step) == 0) == ((lane & size) == 0);

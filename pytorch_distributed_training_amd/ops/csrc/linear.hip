@@ -205,9 +205,9 @@ __device__ __forceinline__ bf16x8 lin_tr_pair(const unsigned char* lo, const uns
 // key = (r & 3) | (r >> 1 & 4), which puts those 8 rows on different banks.
 // PERM: which row of the operand an MFMA row stands for is free.  Row 16 (x >> 2) + 4 j + (x & 3) for row x of block j leaves
 // a lane with 16 neighbouring columns of the result, i.e. with whole 16-byte stores; the key then follows x.
-template <bool TR, int R, int NW, bool PERM, int BK>
+template <bool TR, int R, int NW, bool PERM>
 struct Operand {
-    static constexpr int BYTES = R * BK * 2, PER = BYTES / 1024 / NW, CH = BK / 8;   // CH: chunks of a K-contiguous row
+    static constexpr int BK = LIN_BK, BYTES = R * BK * 2, PER = BYTES / 1024 / NW;
     static_assert(PER >= 1, "every wave takes part in staging");
     static_assert(!(TR && PERM), "the permutation would put a transposing read's rows on the same banks");
     unsigned voff[PER];
@@ -217,13 +217,13 @@ struct Operand {
 
     static __device__ __forceinline__ int key(int row) {
         if (PERM) row = ((row >> 4) & 3) * 4 + (row & 3);
-        return BK == 64 ? (row >> 1) & 7 : (row >> 1) & 2;
+        return (row >> 1) & 7;
     }
     __device__ __forceinline__ static int dma_row(int wave, int lane, int j) {
-        return TR ? (wave * PER + j) * (512 / R) + lane / (R / 8) : (wave * PER + j) * (64 / CH) + lane / CH;
+        return TR ? (wave * PER + j) * (512 / R) + lane / (R / 8) : (wave * PER + j) * 8 + lane / 8;
     }
     __device__ __forceinline__ static int dma_chunk(int lane, int row) {
-        return TR ? (lane % (R / 8)) ^ (2 * ((row & 3) | (row >> 1 & 4))) : (lane % CH) ^ key(row);
+        return TR ? (lane % (R / 8)) ^ (2 * ((row & 3) | (row >> 1 & 4))) : (lane % 8) ^ key(row);
     }
     __device__ __forceinline__ void init(const bf16* x, unsigned long long bytes, int ld, int row0, int k0, int wave, int lane) {
 #pragma unroll
@@ -270,14 +270,15 @@ struct Operand {
     }
 };
 
-template <int BM, int BN, int WM, int WN, int BK, int RING, bool AT, bool BT>
-__global__ __launch_bounds__(WM* WN * 64, BM == 256 || RING > 2 ? 1 : 2) void linear_gemm_kernel(const GemmParams p) {
-    constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
-    constexpr bool PERM = !BT && NI % 4 == 0;
-    typedef Operand<AT, BM, NW, false, BK> A;
-    typedef Operand<BT, BN, NW, PERM, BK> B;
-    constexpr int STAGE = A::BYTES + B::BYTES;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[MI == 8 && NI == 8 ? 5 * A::BYTES : RING * STAGE];
+template <int BM, int BN, int RING, bool AT, bool BT>
+__global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_kernel(const GemmParams p) {
+    constexpr int WM = 2, WN = 2, NW = WM * WN, BK = LIN_BK, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
+    static_assert(BM == BN && RING % 2 == 1 && RING >= 5, "slots of one size, filled in turn");
+    constexpr bool PERM = !BT;
+    typedef Operand<AT, BM, NW, false> A;
+    typedef Operand<BT, BN, NW, PERM> B;
+    constexpr int SLOT = A::BYTES, PER = A::PER;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * SLOT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -310,133 +311,97 @@ __global__ __launch_bounds__(WM* WN * 64, BM == 256 || RING > 2 ? 1 : 2) void li
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    int rem = p.K - k0;                                        // of K, from the stage that is staged next
-    constexpr int PIECES = A::PER + B::PER;
-    const unsigned lds0 = (unsigned)(unsigned long long)(lin_lds_void_t*)smem;
-    if constexpr (MI == 8 && NI == 8) {
-        bf16x8 a0[MI], b0[NI], a1[MI], b1[NI];
-        int rem_b = rem;
-        // slot of operand stage n (a: 2 ks, b: 2 ks + 1) is n mod 5
-        auto half = [&](const bf16x8 (&ac)[MI], const bf16x8 (&bc)[NI], bf16x8 (&an)[MI], bf16x8 (&bn)[NI], int sa, int sb, int kk,
-                        auto&& dma) {
-            const unsigned char *as = smem + sa * A::BYTES, *bs = smem + sb * A::BYTES;
+    // Operand stage n (of a: n = 2 ks, of b: 2 ks + 1) lives in slot n mod RING.  K step ks has two halves of 32 k: the first
+    // multiplies the fragments read last, (ks, 0), reads (ks, 1) and stages n = 2 ks + RING - 1 (of a); a barrier, behind which
+    // the slots of ks are free and those of ks + 1 have landed; the second multiplies (ks, 1), reads (ks + 1, 0) and stages
+    // n = 2 ks + RING (of b).  Reads and DMA go out between the products at an even pace: a wave has its SIMD to itself (or
+    // shares it with one of another workgroup), so whatever is issued in a clump stops the matrix cores.  The stages past the
+    // end of K are staged too, as zeros: no conditions, and the number of DMA in flight is a constant.
+    const unsigned wave_at = (unsigned)(unsigned long long)(lin_lds_void_t*)smem + wave * (PER * 1024);
+    int rem_a = p.K - k0, rem_b = rem_a;                       // of K, from the stage that is staged next
+    bf16x8 a0[MI], b0[NI], a1[MI], b1[NI];
+    constexpr int GROUPS = MI * NI / 4, READS = (MI + NI) / (GROUPS / 2), PACE = GROUPS / PER;
+    static_assert(READS * GROUPS / 2 == MI + NI && PACE * PER == GROUPS, "reads in the first half of the groups");
+    auto half = [&](const bf16x8 (&ac)[MI], const bf16x8 (&bc)[NI], bf16x8 (&an)[MI], bf16x8 (&bn)[NI], int sa, int sb, int kk,
+                    auto&& dma) {
+        const unsigned char *as = smem + sa * SLOT, *bs = smem + sb * SLOT;
 #pragma unroll
-            for (int g = 0; g < 16; ++g) {
-                if (g < 4) {
-                    bn[2 * g] = B::read(bs, wn * WTN, 2 * g, kk, lane);
-                    bn[2 * g + 1] = B::read(bs, wn * WTN, 2 * g + 1, kk, lane);
-                } else if (g < 8) {
-                    an[(2 * g - 8)&7] = A::read(as, wm * WTM, 2 * g - 8, kk, lane);
-                    an[(2 * g - 7)&7] = A::read(as, wm * WTM, 2 * g - 7, kk, lane);
-                }
-                if (g % 2 == 0) dma(g / 2);
+        for (int g = 0; g < GROUPS; ++g) {
+            if (g < GROUPS / 2) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int i = (4 * g + t) / NI, j = (4 * g + t) % NI;
-                    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(bc[j]), "v"(ac[i]));
+                for (int r = g * READS; r < (g + 1) * READS; ++r) {
+                    if (r < NI) bn[r % NI] = B::read(bs, wn * WTN, r % NI, kk, lane);
+                    else an[(r - NI + MI) % MI] = A::read(as, wm * WTM, (r - NI + MI) % MI, kk, lane);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
-        };
-        const unsigned wave_at = lds0 + wave * (A::PER * 1024);
-        auto stage_a = [&](int slot) {
+            if (g % PACE == 0) dma(g / PACE);
+#pragma unroll
+            for (int t = 4 * g; t < 4 * g + 4; ++t)            // (the compiler, left alone, moves half of the sums to VGPRs and spills)
+                asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[t / NI][t % NI]) : "v"(bc[t % NI]), "v"(ac[t / NI]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto stage_a = [&](int slot) {
+        const u32x4 d = a.desc();
+        unsigned m = wave_at + slot * SLOT;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) a.template piece<true>(d, m, rem_a, j, wave, lane);
+        a.next();
+        rem_a -= BK;
+    };
+    auto stage_b = [&](int slot) {
+        const u32x4 d = b.desc();
+        unsigned m = wave_at + slot * SLOT;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) b.template piece<true>(d, m, rem_b, j, wave, lane);
+        b.next();
+        rem_b -= BK;
+    };
+#pragma unroll
+    for (int n = 0; n < RING - 1; n += 2) {
+        stage_a(n);
+        stage_b(n + 1);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 3) * PER) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NI; ++j) b0[j] = B::read(smem + SLOT, wn * WTN, j, 0, lane);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) a0[i] = A::read(smem, wm * WTM, i, 0, lane);
+    int sa = 0;                                                // slot of a's stage ks
+    auto up = [](int s, int n) { return s + n >= RING ? s + n - RING : s + n; };
+    auto k_step = [&](auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        {
             const u32x4 d = a.desc();
-            unsigned m = wave_at + slot * A::BYTES;
-#pragma unroll
-            for (int j = 0; j < A::PER; ++j) a.template piece<true>(d, m, rem, j, wave, lane);
+            unsigned m = wave_at + up(sa, RING - 1) * SLOT;
+            half(a0, b0, a1, b1, sa, up(sa, 1), 1, [&](int j) { a.template piece<TAIL>(d, m, rem_a, j, wave, lane); });
             a.next();
-            rem -= BK;
-        };
-        auto stage_b = [&](int slot) {
-            const u32x4 d = b.desc();
-            unsigned m = wave_at + slot * A::BYTES;
-#pragma unroll
-            for (int j = 0; j < B::PER; ++j) b.template piece<true>(d, m, rem_b, j, wave, lane);
-            b.next();
-            rem_b -= BK;
-        };
-        stage_a(0);
-        stage_b(1);
-        stage_a(2);
-        stage_b(3);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+            rem_a -= BK;
+        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 4) * PER) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < NI; ++j) b0[j] = B::read(smem + A::BYTES, wn * WTN, j, 0, lane);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) a0[i] = A::read(smem, wm * WTM, i, 0, lane);
-        int sa = 0;                                            // slot of a's stage ks
-        auto up = [](int s, int n) { return s + n >= 5 ? s + n - 5 : s + n; };
-        auto k_step = [&](auto tail) {
-            constexpr bool TAIL = decltype(tail)::value;
-            {
-                const u32x4 d = a.desc();
-                unsigned m = wave_at + up(sa, 4) * A::BYTES;
-                half(a0, b0, a1, b1, sa, up(sa, 1), 1, [&](int j) { a.template piece<TAIL>(d, m, rem, j, wave, lane); });
-                a.next();
-                rem -= BK;
-            }
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(A::PER) : "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            {
-                const u32x4 d = b.desc();
-                unsigned m = wave_at + sa * A::BYTES;
-                half(a1, b1, a0, b0, up(sa, 2), up(sa, 3), 0, [&](int j) { b.template piece<TAIL>(d, m, rem_b, j, wave, lane); });
-                b.next();
-                rem_b -= BK;
-            }
-            sa = up(sa, 2);
-        };
-        const int whole = min(rem / BK, nk);                   // steps that stage whole stages
-        int ks = 0;
-        for (; ks < whole; ++ks) k_step(std::integral_constant<bool, false>{});
-        for (; ks < nk; ++ks) k_step(std::integral_constant<bool, true>{});
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
-    } else {
-        bf16x8 af[MI], bfr[NI];
-        unsigned fill = 0, at = 0;                             // slots: staged next, read
-        auto stage = [&]() {
-            const u32x4 da = a.desc(), db = b.desc();
-            unsigned ma = lds0 + fill * STAGE + wave * (A::PER * 1024), mb = lds0 + fill * STAGE + A::BYTES + wave * (B::PER * 1024);
-#pragma unroll
-            for (int j = 0; j < A::PER; ++j) a.template piece<true>(da, ma, rem, j, wave, lane);
-#pragma unroll
-            for (int j = 0; j < B::PER; ++j) b.template piece<true>(db, mb, rem, j, wave, lane);
-            a.next();
+        {
+            const u32x4 d = b.desc();
+            unsigned m = wave_at + sa * SLOT;
+            half(a1, b1, a0, b0, up(sa, 2), up(sa, 3), 0, [&](int j) { b.template piece<TAIL>(d, m, rem_b, j, wave, lane); });
             b.next();
-            rem -= BK;
-            fill = fill == RING - 1 ? 0 : fill + 1;
-        };
-#pragma unroll
-        for (int s = 0; s < RING - 1; ++s) stage();            // (past the end of K: zeros)
-        for (int g = 0; g < nk; ++g) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * PIECES) : "memory");   // this wave's share has landed ...
-            __builtin_amdgcn_s_barrier();                      // ... every wave's has, and the stage before has been read
-            asm volatile("" ::: "memory");
-            stage();
-            const unsigned char* cur = smem + at * STAGE;
-#pragma unroll
-            for (int kk = 0; kk < BK / 32; ++kk) {
-#pragma unroll
-                for (int j = 0; j < NI; ++j) bfr[j] = B::read(cur + A::BYTES, wn * WTN, j, kk, lane);
-#pragma unroll
-                for (int i = 0; i < MI; ++i) af[i] = A::read(cur, wm * WTM, i, kk, lane);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[j], af[i], acc[i][j], 0, 0, 0);
-            }
-            at = at == RING - 1 ? 0 : at + 1;
+            rem_b -= BK;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+        sa = up(sa, 2);
+    };
+    const int whole = min(rem_a / BK, nk);                     // steps that stage whole stages
+    int ks = 0;
+    for (; ks < whole; ++ks) k_step(std::integral_constant<bool, false>{});
+    for (; ks < nk; ++ks) k_step(std::integral_constant<bool, true>{});
+    // every DMA has landed, and the last products are through the pipeline before their sums are read
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
 
     // The sums go through LDS: a lane holds row x = l & 15 of block i and, of block j, four neighbouring columns; out of LDS a
     // thread takes eight neighbouring columns of a row, so that whole rows are loaded (residual) and stored, and what is done to
@@ -619,13 +584,22 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const bf16* __restrict__
     float* out = sums + (long long)blockIdx.y * N + c;
     *out = add ? *out + t : t;
 }
+// 64 columns a block, its four waves share the parts; the waves' sums are added in order
 __global__ __launch_bounds__(256) void linear_sums_kernel(const float* __restrict__ part, float* __restrict__ out, int N,
                                                           int parts, int add) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
     float t = 0.0f;
-    for (int i = 0; i < parts; ++i) t += part[(long long)i * N + c];
-    out[c] = add ? out[c] + t : t;
+    if (c < N) {
+#pragma unroll 8
+        for (int i = wave; i < parts; i += 4) t += part[(long long)i * N + c];
+    }
+    red[wave][lane] = t;
+    __syncthreads();
+    if (wave == 0 && c < N) {
+        t = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+        out[c] = add ? out[c] + t : t;
+    }
 }
 
 // rows of any stride and alignment -> rows of ldp columns (a multiple of 8), zeros behind the last one
@@ -658,7 +632,12 @@ struct Plan {
 static Plan plan_of(long long M, long long N, long long K) {
     Plan q;
     const int nk = cdiv(K, LIN_BK);
-    q.big = (long long)cdiv(M, 256) * cdiv(N, 256) >= LIN_CUS * 3 / 4;
+    // 256 x 256 tiles run one to a CU and take about 16 us plus 1.45 us a step of 64 each (most of the 16 us: nothing covers
+    // their prologue and their 64 Ki results); 128 x 128 tiles run two to a CU and take 2.8 + 0.43 us per tile and CU.
+    // 4096 x 16384 x 4096: 418 us against 580; x 1024: 156 / 152; x 128: 75 / 56; 2048 x 4096 x 4096 (128 tiles of 256): 91 / 63.
+    const long long big = (long long)cdiv((long long)cdiv(M, 256) * cdiv(N, 256), LIN_CUS) * (1600 + 145ll * nk);
+    const long long small = (long long)cdiv((long long)cdiv(M, 128) * cdiv(N, 128), LIN_CUS) * (275 + 43ll * nk);
+    q.big = big < small;
     const int t = q.big ? 256 : 128;
     q.tiles_m = cdiv(M, t), q.tiles_n = cdiv(N, t);
     const long long tiles = (long long)q.tiles_m * q.tiles_n;
@@ -695,9 +674,10 @@ static int launch_gemm(const bf16* a, const bf16* b, unsigned long long a_bytes,
         p.ep.mode = OUT_PART, p.ep.ws = ws;
     }
     const dim3 grid(q.tiles_m * q.tiles_n * q.splits);
-    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 2, 2, 64, 2, AT, BT>), grid, dim3(256), 0, s, p);
-    else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, 64, 4, AT, BT>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 2, 2, 64, 2, AT, BT>), grid, dim3(256), 0, s, p);
+    // 128 x 128 tiles: two workgroups of 80 KB on a CU where there are that many, else one with a deeper ring
+    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, AT, BT>), grid, dim3(256), 0, s, p);
+    else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
     if (q.splits > 1) {
         p.ep.mode = mode;
         hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((ep.n_pad + 7) / 8) * ep.M, 256)), dim3(256), 0, s, p.ep, q.splits);
@@ -775,7 +755,7 @@ PDT_API int pdt_linear_dz(const void* dy, const void* z, void* dz, void* dbias, 
                        act == LIN_NONE ? nullptr : static_cast<const bf16*>(z), static_cast<bf16*>(dz), out, ldy, ldz, lddz, M, N,
                        act, cdiv(M, parts), parts > 1 ? 0 : add);
     if (parts > 1)
-        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 256)), dim3(256), 0, s, out, static_cast<float*>(dbias), N, parts, add);
+        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 64)), dim3(256), 0, s, out, static_cast<float*>(dbias), N, parts, add);
     return pdt_launch_status();
 }
 

@@ -654,43 +654,47 @@ def linear_act_bwd(a: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, z: Option
 MAX_TOP = 512                # slots per row
 MAX_CLASSES = 262144
 _LOGIT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_INDEX_DTYPES = (torch.int32, torch.int64)
 
 
-def _check_logits(what: str, logits: torch.Tensor, temperature: float) -> None:
+def _check_logits(what: str, logits: torch.Tensor, temperature: float):
+    shape = logits.shape
     if logits.dtype not in _LOGIT_DTYPES:
         raise TypeError(f"{what}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_CLASSES:
-        raise ValueError(f"{what}: logits must be [rows, classes] with 1 to {MAX_CLASSES} classes, got {tuple(logits.shape)}")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_CLASSES:
+        raise ValueError(f"{what}: logits must be [rows, classes] with 1 to {MAX_CLASSES} classes, got {tuple(shape)}")
+    if logits.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f"{what}: logits must have unit column stride")
     if not 1e-3 <= temperature <= 1e3:
         raise ValueError(f"{what}: temperature must lie in [0.001, 1000], got {temperature}")
+    return shape
 
 
 def check_top_logits(logits: torch.Tensor, k: int, temperature: float) -> None:
-    _check_logits("top_logits", logits, temperature)
-    if not 1 <= k <= min(MAX_TOP, logits.shape[1]):
-        raise ValueError(f"top_logits: k must lie in [1, {min(MAX_TOP, logits.shape[1])}], got {k}")
+    N = _check_logits("top_logits", logits, temperature)[1]
+    if not 1 <= k <= min(MAX_TOP, N):
+        raise ValueError(f"top_logits: k must lie in [1, {min(MAX_TOP, N)}], got {k}")
+
+
+def _check_per_row(name: str, t: torch.Tensor, dtypes, B: int) -> None:
+    if t.dtype not in dtypes:
+        raise TypeError(f"distill_ce: {name} must be one of {dtypes}, got {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != B or not t.is_contiguous():
+        raise ValueError(f"distill_ce: {name} must be [{B}] and contiguous, got {tuple(t.shape)}")
 
 
 def check_distill_ce(logits, labels, values, indices, temperature: float, alpha: float, lse) -> None:
-    _check_logits("distill_ce", logits, temperature)
-    B = logits.shape[0]
-    if values.dtype not in _LOGIT_DTYPES or indices.dtype not in (torch.int32, torch.int64):
+    B = _check_logits("distill_ce", logits, temperature)[0]
+    shape = values.shape
+    if values.dtype not in _LOGIT_DTYPES or indices.dtype not in _INDEX_DTYPES:
         raise TypeError(f"distill_ce: values must be bf16 / fp16 / fp32 and indices int32 / int64, got {values.dtype}, {indices.dtype}")
-    if values.dim() != 2 or values.shape[0] != B or values.shape != indices.shape or not 1 <= values.shape[1] <= MAX_TOP:
+    if len(shape) != 2 or shape[0] != B or shape != indices.shape or not 1 <= shape[1] <= MAX_TOP:
         raise ValueError(f"distill_ce: values and indices must both be [{B}, k] with k in [1, {MAX_TOP}], got "
-                         f"{tuple(values.shape)}, {tuple(indices.shape)}")
+                         f"{tuple(shape)}, {tuple(indices.shape)}")
     if labels is not None:
-        if labels.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"distill_ce: labels must be int32 / int64, got {labels.dtype}")
-        if labels.shape != (B,) or (B > 1 and labels.stride(0) != 1):
-            raise ValueError(f"distill_ce: labels must be [{B}] and contiguous, got {tuple(labels.shape)}")
+        _check_per_row("labels", labels, _INDEX_DTYPES, B)
     if lse is not None:
-        if lse.dtype != torch.float32:
-            raise TypeError(f"distill_ce: lse must be fp32, got {lse.dtype}")
-        if lse.shape != (B,) or (B > 1 and lse.stride(0) != 1):
-            raise ValueError(f"distill_ce: lse must be [{B}] and contiguous, got {tuple(lse.shape)}")
+        _check_per_row("lse", lse, (torch.float32,), B)
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"distill_ce: alpha must lie in [0, 1], got {alpha}")
 
