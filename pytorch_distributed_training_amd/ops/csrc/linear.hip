@@ -270,15 +270,15 @@ struct Operand {
     }
 };
 
+// tile `block` of `p`; smem: RING slots
 template <int BM, int BN, int RING, bool AT, bool BT>
-__global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_kernel(const GemmParams p) {
+__device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, unsigned char* smem) {
     constexpr int WM = 2, WN = 2, NW = WM * WN, BK = LIN_BK, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
     static_assert(BM == BN && RING % 2 == 1 && RING >= 5, "slots of one size, filled in turn");
     constexpr bool PERM = !BT;
     typedef Operand<AT, BM, NW, false> A;
     typedef Operand<BT, BN, NW, PERM> B;
     constexpr int SLOT = A::BYTES, PER = A::PER;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * SLOT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_
     int m0, n0, split;
     {
         const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
-        const int xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
-        int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (blockIdx.x >> 3);
+        const int xcd = block & 7, q = total >> 3, r = total & 7;
+        int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (block >> 3);
         split = id / per;
         id -= split * per;
         const int g = id / (GROUP * p.tiles_n), rows = min(GROUP, p.tiles_m - g * GROUP);
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_
     // tile: as long as 40 K steps.)  16-byte chunk c of a row is kept at c ^ x: the 16 rows of a write fall on different banks.
     const Epilogue& ep = p.ep;
     constexpr int PI = MI < 4 ? MI : 4, ROWS = WM * PI * 16, NT = NW * 64, COLS8 = BN / 8;
-    static_assert(ROWS * BN * 4 <= sizeof(smem), "a pass fits");
+    static_assert(ROWS * BN * 4 <= RING * SLOT, "a pass fits");
     const int x = lane & 15, fq = lane >> 4;
     const int n = n0 + (int)(threadIdx.x % COLS8) * 8;
     float bias[8];
@@ -441,6 +441,20 @@ __global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_
             }
         }
     }
+}
+
+template <int BM, int BN, int RING, bool AT, bool BT>
+__global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_kernel(const GemmParams p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * BM * LIN_BK * 2];
+    gemm_tile<BM, BN, RING, AT, BT>(p, blockIdx.x, smem);
+}
+
+// Both gradients of a layer in one launch: dw = dz^T a in the first workgroups, da = dz w in the rest.  Where neither has
+// tiles enough for the chip, each alone would leave CUs idle or pay for a split of its K.
+__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int first) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[5 * 128 * LIN_BK * 2];
+    if ((int)blockIdx.x < first) gemm_tile<128, 128, 5, true, true>(dw, blockIdx.x, smem);
+    else gemm_tile<128, 128, 5, false, true>(da, blockIdx.x - first, smem);
 }
 
 // Joins the partial sums of a product whose K range was split (too few tiles for the chip), in slab order, and does what the
@@ -602,33 +616,50 @@ __global__ __launch_bounds__(256) void linear_sums_kernel(const float* __restric
     }
 }
 
-// rows of any stride and alignment -> rows of ldp columns (a multiple of 8), zeros behind the last one
-__global__ __launch_bounds__(256) void linear_pack_kernel(const bf16* __restrict__ src, bf16* __restrict__ dst, long long ld,
-                                                          int ldp, int rows, int cols) {
-    const int vecs = ldp / 8;
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+// rows of any stride and alignment -> rows of ldp columns (a multiple of 8), zeros behind the last one; one or two matrices
+struct PackJob {
+    const bf16* src;
+    bf16* dst;
+    long long ld;
+    int ldp, rows, cols, blocks;
+};
+__global__ __launch_bounds__(256) void linear_pack_kernel(const PackJob j0, const PackJob j1) {
+    const bool second = (int)blockIdx.x >= j0.blocks;
+    const PackJob& j = second ? j1 : j0;
+    const int vecs = j.ldp / 8;
+    const long long t = (long long)(blockIdx.x - (second ? j0.blocks : 0)) * 256 + threadIdx.x;
     const long long row = t / vecs;
     const int c = (int)(t % vecs) * 8;
-    if (row >= rows) return;
-    const bf16* s = src + row * ld + c;
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (c + 8 <= cols) v = *reinterpret_cast<const u32x4_a2*>(s);
+    if (row >= j.rows) return;
+    const bf16* s = j.src + row * j.ld + c;
+    u32x4 v;
+    if (c + 8 <= j.cols) v = *reinterpret_cast<const u32x4_a2*>(s);
     else {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = c + e < cols ? (float)s[e] : 0.0f;
+        for (int e = 0; e < 8; ++e) f[e] = c + e < j.cols ? (float)s[e] : 0.0f;
         v = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
     }
-    *reinterpret_cast<u32x4*>(dst + row * ldp + c) = v;
+    *reinterpret_cast<u32x4*>(j.dst + row * j.ldp + c) = v;
 }
 
 // ------------------------------------------------------------------------------------------ launchers
 #define LIN_MAX_LD (1 << 22)           // 256 rows of an operand stay below 2 GiB of 32-bit offsets
 #define LIN_CUS 256
 
+// How a product is cut up.  Costs are in units of 10 ns.
 struct Plan {
     int big, splits, steps, tiles_m, tiles_n;
+    long long cost;
+    long long blocks() const { return (long long)tiles_m * tiles_n * splits; }
 };
+static void cut(Plan& q, int tile, long long M, long long N, int nk, int splits) {
+    q.big = tile == 256, q.tiles_m = cdiv(M, tile), q.tiles_n = cdiv(N, tile);
+    q.steps = cdiv(nk, splits), q.splits = cdiv(nk, q.steps);
+}
+// joining partial sums: 4 us and their way through memory at 4.5 TB/s
+static long long join_cost(long long M, long long N, int splits) { return splits > 1 ? 400 + splits * M * N * 8 / 45000 : 0; }
+
 static Plan plan_of(long long M, long long N, long long K) {
     Plan q;
     const int nk = cdiv(K, LIN_BK);
@@ -636,53 +667,115 @@ static Plan plan_of(long long M, long long N, long long K) {
     // their prologue and their 64 Ki results); 128 x 128 tiles run two to a CU and take 2.8 + 0.43 us per tile and CU.
     // 4096 x 16384 x 4096: 418 us against 580; x 1024: 156 / 152; x 128: 75 / 56; 2048 x 4096 x 4096 (128 tiles of 256): 91 / 63.
     const long long big = (long long)cdiv((long long)cdiv(M, 256) * cdiv(N, 256), LIN_CUS) * (1600 + 145ll * nk);
-    const long long small = (long long)cdiv((long long)cdiv(M, 128) * cdiv(N, 128), LIN_CUS) * (275 + 43ll * nk);
-    q.big = big < small;
-    const int t = q.big ? 256 : 128;
-    q.tiles_m = cdiv(M, t), q.tiles_n = cdiv(N, t);
-    const long long tiles = (long long)q.tiles_m * q.tiles_n;
-    q.splits = 1;
-    if (!q.big && tiles < LIN_CUS) q.splits = (int)max(1ll, min(LIN_CUS / tiles, (long long)nk / 4));
-    q.steps = cdiv(nk, q.splits);
-    q.splits = cdiv(nk, q.steps);
+    const long long tiles = (long long)cdiv(M, 128) * cdiv(N, 128), small = (long long)cdiv(tiles, LIN_CUS) * (275 + 43ll * nk);
+    q.cost = big < small ? big : small;
+    int splits = 1;
+    // K ranges, while one workgroup per CU holds them: a step of a lone 128 x 128 workgroup takes 0.56 us (1000 x 2048 x 1536,
+    // 128 tiles: one range 19 us, two 24; 64 x 4096 x 4096, 32 tiles: one 40 us, eight 16).
+    if (big >= small && tiles < LIN_CUS) {
+        q.cost = 275 + 56ll * nk;
+        for (int s = 2; s <= LIN_CUS / tiles && s <= nk / 2; ++s) {
+            const long long cost = 275 + 56ll * cdiv(nk, s) + join_cost(M, N, s);
+            if (cost < q.cost) q.cost = cost, splits = s;
+        }
+    }
+    cut(q, big < small ? 256 : 128, M, N, nk, splits);
     return q;
 }
 
-// floats of workspace that a product needs
-PDT_API long long pdt_linear_workspace(long long M, long long N, long long K) {
-    if (M < 1 || N < 1 || K < 1) return 0;
-    const Plan q = plan_of(M, N, K);
-    return q.splits > 1 ? q.splits * M * slab_ld((int)N) : 0;
+// Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then.  Two workgroups on a CU take
+// 0.75 us a step where the chip is not full, and the same 0.43 us per tile and CU where it is; a launch of its own costs about
+// 2 us.  1536 x 2048 x 1000: PAIR_US us against SOLO_US.
+static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da) {
+    dw = plan_of(N, K, M), da = plan_of(M, K, N);
+    const long long tw = (long long)cdiv(N, 128) * cdiv(K, 128), ta = (long long)cdiv(M, 128) * cdiv(K, 128);
+    const int nw = cdiv(M, LIN_BK), na = cdiv(N, LIN_BK);
+    if (tw + ta > 8 * LIN_CUS) return false;                   // each fills the chip
+    long long best = dw.cost + da.cost + 200;
+    int best_w = 0, best_a = 0;
+    for (int sw = 1; sw == 1 || (sw <= 16 && sw <= nw / 2 && sw * tw <= 2 * LIN_CUS); ++sw)
+        for (int sa = 1; sa == 1 || (sa <= 16 && sa <= na / 2 && sa * ta <= 2 * LIN_CUS); ++sa) {
+            const int kw = cdiv(nw, sw), ka = cdiv(na, sa), k = kw > ka ? kw : ka;
+            const long long blocks = tw * sw + ta * sa;
+            const long long work = (tw * sw * (275 + 43ll * kw) + ta * sa * (275 + 43ll * ka)) / LIN_CUS;
+            const long long one = 275 + (blocks <= LIN_CUS ? 56ll : 75ll) * k, rounds = blocks > 2 * LIN_CUS ? work + one / 2 : 0;
+            long long cost = work > one ? work : one;
+            cost = (cost > rounds ? cost : rounds) + join_cost(N, K, sw) + join_cost(M, K, sa);
+            if (cost < best) best = cost, best_w = sw, best_a = sa;
+        }
+    if (!best_w) return false;
+    cut(dw, 128, N, K, nw, best_w), cut(da, 128, M, K, na, best_a);
+    return true;
 }
 
 static bool aligned16(const void* p) { return ((unsigned long long)p & 15) == 0; }
+static int pad8(int n) { return (n + 7) / 8 * 8; }
+static int pad64(int n) { return (n + 63) / 64 * 64; }
 
-template <bool AT, bool BT>
-static int launch_gemm(const bf16* a, const bf16* b, unsigned long long a_bytes, unsigned long long b_bytes, long long lda,
-                       long long ldb, int K, Epilogue ep, float* ws, hipStream_t s) {
-    if (!aligned16(a) || !aligned16(b) || lda % 8 || ldb % 8 || lda >= LIN_MAX_LD || ldb >= LIN_MAX_LD) return -2;
-    if ((!AT || !BT) && K % 8) return -2;
-    const Plan q = plan_of(ep.M, ep.N, K);
-    if ((long long)q.tiles_m * q.tiles_n * q.splits > 0x7fffffffll) return -1;
-    GemmParams p;
-    p.a = a, p.b = b, p.a_bytes = a_bytes, p.b_bytes = b_bytes, p.lda = (int)lda, p.ldb = (int)ldb, p.K = K;
-    p.splits = q.splits, p.steps = q.steps, p.tiles_m = q.tiles_m, p.tiles_n = q.tiles_n;
-    const int mode = ep.mode;
-    p.ep = ep;
-    if (q.splits > 1) {
-        if (!ws) return -3;
-        p.ep.mode = OUT_PART, p.ep.ws = ws;
+// An operand of the tile kernel: rows start at 16-byte boundaries and hold a multiple of 8 columns (zeros behind the last
+// one; a descriptor that ended inside a 4-byte word would return that word's valid half as zero too).
+struct Matrix {
+    const bf16* p;
+    long long ld;
+    int rows, cols;
+    bool fits() const { return cols % 8 == 0 && ld % 8 == 0 && ld >= cols && ld < LIN_MAX_LD && aligned16(p); }
+    unsigned long long bytes() const {
+        return ((unsigned long long)(rows - 1) * (unsigned long long)ld + (unsigned long long)pad8(cols)) * 2ull;
     }
-    const dim3 grid(q.tiles_m * q.tiles_n * q.splits);
+};
+
+// Regions of a call's workspace, one behind the other; without memory (null) it only adds up what is needed.
+struct Arena {
+    unsigned char* base;
+    unsigned long long used = 0;
+    void* take(unsigned long long bytes) {
+        void* p = base ? base + used : nullptr;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// ``m`` itself, or the place of its padded copy; the copies are made by one launch
+static Matrix operand(const Matrix& m, Arena& ws, PackJob& job) {
+    job.blocks = 0;
+    if (m.fits()) return m;
+    const int ldp = pad8(m.cols);
+    bf16* dst = static_cast<bf16*>(ws.take((unsigned long long)m.rows * ldp * 2));
+    job.src = m.p, job.dst = dst, job.ld = m.ld, job.ldp = ldp, job.rows = m.rows, job.cols = m.cols;
+    job.blocks = cdiv((long long)m.rows * (ldp / 8), 256);
+    return Matrix{dst, ldp, m.rows, m.cols};
+}
+static void launch_pack(const PackJob& j0, const PackJob& j1, hipStream_t s) {
+    if (j0.blocks + j1.blocks > 0)
+        hipLaunchKernelGGL(linear_pack_kernel, dim3(j0.blocks + j1.blocks), dim3(256), 0, s, j0, j1);
+}
+
+static unsigned long long slab_bytes(const Plan& q, long long M, int N) {
+    return q.splits > 1 ? (unsigned long long)q.splits * M * slab_ld(N) * 4ull : 0ull;
+}
+
+static GemmParams gemm_params(const Plan& q, const Matrix& a, const Matrix& b, int K, const Epilogue& ep, float* slabs) {
+    GemmParams p;
+    p.a = a.p, p.b = b.p, p.a_bytes = a.bytes(), p.b_bytes = b.bytes(), p.lda = (int)a.ld, p.ldb = (int)b.ld, p.K = K;
+    p.splits = q.splits, p.steps = q.steps, p.tiles_m = q.tiles_m, p.tiles_n = q.tiles_n;
+    p.ep = ep;
+    if (q.splits > 1) p.ep.mode = OUT_PART, p.ep.ws = slabs;
+    return p;
+}
+static void launch_join(const GemmParams& p, int mode, hipStream_t s) {
+    if (p.splits < 2) return;
+    Epilogue e = p.ep;
+    e.mode = mode;
+    hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((e.n_pad + 7) / 8) * e.M, 256)), dim3(256), 0, s, e, p.splits);
+}
+template <bool AT, bool BT>
+static void launch_gemm(const Plan& q, const GemmParams& p, int mode, hipStream_t s) {
+    const dim3 grid((unsigned)q.blocks());
     // 128 x 128 tiles: two workgroups of 80 KB on a CU where there are that many, else one with a deeper ring
     if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, AT, BT>), grid, dim3(256), 0, s, p);
     else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
-    if (q.splits > 1) {
-        p.ep.mode = mode;
-        hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((ep.n_pad + 7) / 8) * ep.M, 256)), dim3(256), 0, s, p.ep, q.splits);
-    }
-    return pdt_launch_status();
+    launch_join(p, mode, s);
 }
 
 static Epilogue plain_epilogue(void* out, int mode, int M, int N, long long ldo) {
@@ -692,77 +785,138 @@ static Epilogue plain_epilogue(void* out, int mode, int M, int N, long long ldo)
     e.vec = ldo % 8 == 0 && aligned16(out);
     return e;
 }
-static int pad8(int n) { return (n + 7) / 8 * 8; }
-// Memory of an operand: its rows hold a multiple of 8 columns (zeros behind the last one).  A descriptor that ended inside a
-// 4-byte word would return that word's valid half as zero too.
-static unsigned long long span_bytes(long long rows, int cols, long long ld) {
-    return ((unsigned long long)(rows - 1) * (unsigned long long)ld + (unsigned long long)pad8(cols)) * 2ull;
+
+// Whether a forward product goes to the kernel for few rows, which reads a once per 16 rows of w: 4096 x 4096 with 32 rows
+// 14.6 us against 15.5 with tiles, with 64 rows 23.1 / 16.8; 16384 x 4096 with 4 rows 31.9 / 37.9, with 16 rows 40.0 / 38.2.
+// Rows that tiles need copied first (777 x 1021: 6 us more) leave it ahead for longer.
+static bool few_rows(int M, int N, int K, bool copies) {
+    return M <= 64 && (long long)M * N * K <= (copies ? 1ll << 31 : 1ll << 29);
+}
+struct FwdPlan {
+    Matrix a, w;
+    PackJob ja, jw;
+    Plan plan;
+    float* slabs;
+    bool few;
+    unsigned long long bytes;
+};
+static FwdPlan plan_fwd(const void* a, const void* w, void* ws, int M, int N, int K, long long lda, long long ldw) {
+    FwdPlan f;
+    f.a = Matrix{static_cast<const bf16*>(a), lda, M, K}, f.w = Matrix{static_cast<const bf16*>(w), ldw, N, K};
+    f.few = few_rows(M, N, K, !f.a.fits() || !f.w.fits());
+    f.slabs = nullptr, f.ja.blocks = f.jw.blocks = 0;
+    Arena mem{static_cast<unsigned char*>(ws)};
+    if (!f.few) {
+        f.a = operand(f.a, mem, f.ja), f.w = operand(f.w, mem, f.jw);
+        f.plan = plan_of(M, N, pad8(K));
+        f.slabs = static_cast<float*>(mem.take(slab_bytes(f.plan, M, N)));
+    }
+    f.bytes = mem.used;
+    return f;
 }
 
-// Status -1: sizes, -2: alignment, -3: a workspace is needed.  The tile kernel's operands have rows that start at 16-byte
-// boundaries and are padded to a multiple of 8 columns, with zeros.
-// few: take the kernel for few rows (M <= 64), which needs no alignment.
+// bytes of workspace that pdt_linear_fwd needs for these operands
+PDT_API long long pdt_linear_fwd_workspace(const void* a, const void* w, int M, int N, int K, long long lda, long long ldw) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    return (long long)plan_fwd(a, w, nullptr, M, N, K, lda, ldw).bytes;
+}
+
+// Status -1: sizes, -3: a workspace is needed (nothing was launched).  y and z: rows of ldo = N rounded up to 64 columns.
 PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const void* res, void* y, void* z, void* ws, int M, int N,
-                           int K, long long lda, long long ldw, long long ldr, int ldo, int act, int few, hipStream_t s) {
-    if (M < 0 || N < 1 || K < 1 || ldo < N || ldo % 64 || act < 0 || act > LIN_SILU || (few && M > 64)) return -1;
+                           int K, long long lda, long long ldw, long long ldr, int ldo, int act, hipStream_t s) {
+    if (M < 0 || N < 1 || K < 1 || ldo != pad64(N) || act < 0 || act > LIN_SILU) return -1;
     if (M == 0) return 0;
+    const FwdPlan f = plan_fwd(a, w, ws, M, N, K, lda, ldw);
+    if (f.bytes > 0 && !ws) return -3;
     Epilogue e = plain_epilogue(y, OUT_BF16, M, N, ldo);
     e.z = static_cast<bf16*>(z), e.bias = static_cast<const float*>(bias), e.res = static_cast<const bf16*>(res);
-    e.ldr = ldr, e.act = act, e.n_pad = (N + 63) / 64 * 64;
-    const bf16 *ap = static_cast<const bf16*>(a), *wp = static_cast<const bf16*>(w);
-    if (few) {
+    e.ldr = ldr, e.act = act, e.n_pad = ldo;
+    if (f.few) {
         const dim3 grid(cdiv(N, 16));
-        if (M <= 16) hipLaunchKernelGGL((linear_rows_kernel<1, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
-        else if (M <= 32) hipLaunchKernelGGL((linear_rows_kernel<2, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
-        else hipLaunchKernelGGL((linear_rows_kernel<4, 8>), grid, dim3(512), 0, s, ap, wp, lda, ldw, K, e);
+        if (M <= 16) hipLaunchKernelGGL((linear_rows_kernel<1, 8>), grid, dim3(512), 0, s, f.a.p, f.w.p, lda, ldw, K, e);
+        else if (M <= 32) hipLaunchKernelGGL((linear_rows_kernel<2, 8>), grid, dim3(512), 0, s, f.a.p, f.w.p, lda, ldw, K, e);
+        else hipLaunchKernelGGL((linear_rows_kernel<4, 8>), grid, dim3(512), 0, s, f.a.p, f.w.p, lda, ldw, K, e);
         return pdt_launch_status();
     }
-    if (lda < pad8(K) || ldw < pad8(K)) return -2;
-    return launch_gemm<false, false>(ap, wp, span_bytes(M, K, lda), span_bytes(N, K, ldw), lda, ldw, K, e, static_cast<float*>(ws), s);
-}
-
-// da[M][K] = dz[M][N] w[N][K]
-PDT_API int pdt_linear_da(const void* dz, const void* w, void* da, void* ws, int M, int N, int K, long long lddz, long long ldw,
-                          long long ldda, hipStream_t s) {
-    if (M < 0 || N < 1 || K < 1 || ldda < K) return -1;
-    if (M == 0) return 0;
-    if (lddz < pad8(N) || ldw < pad8(K)) return -2;
-    return launch_gemm<false, true>(static_cast<const bf16*>(dz), static_cast<const bf16*>(w), span_bytes(M, N, lddz),
-                                    span_bytes(N, K, ldw), lddz, ldw, pad8(N), plain_epilogue(da, OUT_BF16, M, K, ldda),
-                                    static_cast<float*>(ws), s);
-}
-
-// dw[N][K] (bf16, or fp32 added to) = dz[M][N]^T a[M][K]
-PDT_API int pdt_linear_dw(const void* dz, const void* a, void* dw, void* ws, int M, int N, int K, long long lddz, long long lda,
-                          long long lddw, int add, hipStream_t s) {
-    if (M < 1 || N < 1 || K < 1 || lddw < K) return -1;
-    if (lddz < pad8(N) || lda < pad8(K)) return -2;
-    return launch_gemm<true, true>(static_cast<const bf16*>(dz), static_cast<const bf16*>(a), span_bytes(M, N, lddz),
-                                   span_bytes(M, K, lda), lddz, lda, M, plain_epilogue(dw, add ? OUT_ADD : OUT_BF16, N, K, lddw),
-                                   static_cast<float*>(ws), s);
-}
-
-// dz = dy act'(z) (dz may be null when act is none) and dbias (+)= its column sums; parts: row blocks, ws: parts * N floats
-// when parts > 1.
-PDT_API int pdt_linear_dz(const void* dy, const void* z, void* dz, void* dbias, void* ws, int M, int N, long long ldy, long long ldz,
-                          int lddz, int act, int parts, int add, hipStream_t s) {
-    if (M < 1 || N < 1 || act < 0 || act > LIN_SILU || parts < 1 || parts > 65535 || (act != LIN_NONE && (!z || !dz))) return -1;
-    if (dz && (lddz < pad8(N) || lddz % 8 || !aligned16(dz))) return -2;
-    if (parts > 1 && !ws) return -3;
-    const int cols = dz ? lddz : N;
-    float* out = static_cast<float*>(parts > 1 ? ws : dbias);
-    hipLaunchKernelGGL(linear_dz_kernel, dim3(cdiv(cols, 256), parts), dim3(256), 0, s, static_cast<const bf16*>(dy),
-                       act == LIN_NONE ? nullptr : static_cast<const bf16*>(z), static_cast<bf16*>(dz), out, ldy, ldz, lddz, M, N,
-                       act, cdiv(M, parts), parts > 1 ? 0 : add);
-    if (parts > 1)
-        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 64)), dim3(256), 0, s, out, static_cast<float*>(dbias), N, parts, add);
+    if (f.plan.blocks() > 0x7fffffffll) return -1;
+    launch_pack(f.ja, f.jw, s);
+    launch_gemm<false, false>(f.plan, gemm_params(f.plan, f.a, f.w, pad8(K), e, f.slabs), OUT_BF16, s);
     return pdt_launch_status();
 }
 
-PDT_API int pdt_linear_pack(const void* src, void* dst, long long ld, int ldp, int rows, int cols, hipStream_t s) {
-    if (rows < 0 || cols < 1 || ldp % 8 || ldp < cols || !aligned16(dst)) return -1;
-    if (rows == 0) return 0;
-    hipLaunchKernelGGL(linear_pack_kernel, dim3(cdiv((long long)rows * (ldp / 8), 256)), dim3(256), 0, s,
-                       static_cast<const bf16*>(src), static_cast<bf16*>(dst), ld, ldp, rows, cols);
+struct BwdPlan {
+    Matrix dz, a, w;
+    PackJob ja, jw;
+    bf16* dz_out;             // where dz is written, or null: dy is the operand as it is
+    float *parts, *slabs_w, *slabs_a;
+    int n_parts;
+    Plan pw, pa;
+    bool pair;
+    unsigned long long bytes;
+};
+static BwdPlan plan_bwd(const void* dy, const void* a, const void* w, void* ws, int M, int N, int K, long long lddy, long long lda,
+                        long long ldw, int act, int need_da) {
+    BwdPlan f;
+    Arena mem{static_cast<unsigned char*>(ws)};
+    f.dz = Matrix{static_cast<const bf16*>(dy), lddy, M, N}, f.dz_out = nullptr;
+    if (act != LIN_NONE || !f.dz.fits()) {
+        f.dz_out = static_cast<bf16*>(mem.take((unsigned long long)M * pad64(N) * 2));
+        f.dz = Matrix{f.dz_out, pad64(N), M, N};
+    }
+    f.a = operand(Matrix{static_cast<const bf16*>(a), lda, M, K}, mem, f.ja);
+    f.jw.blocks = 0;
+    if (need_da) f.w = operand(Matrix{static_cast<const bf16*>(w), ldw, N, K}, mem, f.jw);
+    // row blocks of the bias gradient: about four workgroups per CU, each with at least 32 rows
+    const int cap = 1024 * 256 / pad64(N);
+    f.n_parts = cdiv(M, 32) < cap ? cdiv(M, 32) : (cap > 0 ? cap : 1);
+    f.parts = f.n_parts > 1 ? static_cast<float*>(mem.take((unsigned long long)f.n_parts * N * 4)) : nullptr;
+    f.pair = need_da && plan_pair(M, N, K, f.pw, f.pa);
+    if (!f.pair) {
+        f.pw = plan_of(N, K, M);
+        if (need_da) f.pa = plan_of(M, K, pad8(N));
+    }
+    const unsigned long long sw = slab_bytes(f.pw, N, K), sa = need_da ? slab_bytes(f.pa, M, K) : 0ull;
+    f.slabs_w = static_cast<float*>(mem.take(sw));
+    f.slabs_a = static_cast<float*>(f.pair ? mem.take(sa) : f.slabs_w);
+    if (!f.pair && sa > sw) mem.take(sa - sw);                 // (one product after the other: the same place)
+    f.bytes = mem.used;
+    return f;
+}
+
+PDT_API long long pdt_linear_bwd_workspace(const void* dy, const void* a, const void* w, int M, int N, int K, long long lddy,
+                                           long long lda, long long ldw, int act, int need_da) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    return (long long)plan_bwd(dy, a, w, nullptr, M, N, K, lddy, lda, ldw, act, need_da).bytes;
+}
+
+// dz = dy act'(z);  dbias (+)= its column sums;  da = dz w (da null: not wanted);  dw (bf16, or fp32 added to) = dz^T a.
+// Status as above.
+PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const void* w, void* da, void* dw, void* dbias, void* ws,
+                           int M, int N, int K, long long lddy, long long ldz, long long lda, long long ldw, long long lddw, int act,
+                           int add_w, int add_b, hipStream_t s) {
+    if (M < 1 || N < 1 || K < 1 || lddw < K || lddw > 0x7fffffffll || act < 0 || act > LIN_SILU || (act != LIN_NONE && !z)) return -1;
+    const BwdPlan f = plan_bwd(dy, a, w, ws, M, N, K, lddy, lda, ldw, act, da != nullptr);
+    if (f.pw.blocks() > 0x7fffffffll || (da && f.pa.blocks() > 0x7fffffffll)) return -1;
+    if (f.bytes > 0 && !ws) return -3;
+    const int cols = f.dz_out ? pad64(N) : N;
+    hipLaunchKernelGGL(linear_dz_kernel, dim3(cdiv(cols, 256), f.n_parts), dim3(256), 0, s, static_cast<const bf16*>(dy),
+                       act == LIN_NONE ? nullptr : static_cast<const bf16*>(z), f.dz_out,
+                       f.n_parts > 1 ? f.parts : static_cast<float*>(dbias), lddy, ldz, (int)f.dz.ld, M, N, act, cdiv(M, f.n_parts),
+                       f.n_parts > 1 ? 0 : add_b);
+    if (f.n_parts > 1)
+        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 64)), dim3(256), 0, s, f.parts, static_cast<float*>(dbias), N, f.n_parts, add_b);
+    launch_pack(f.ja, f.jw, s);
+    const int mode = add_w ? OUT_ADD : OUT_BF16;
+    const GemmParams pw = gemm_params(f.pw, f.dz, f.a, M, plain_epilogue(dw, mode, N, K, lddw), f.slabs_w);
+    GemmParams pa;
+    if (da) pa = gemm_params(f.pa, f.dz, f.w, pad8(N), plain_epilogue(da, OUT_BF16, M, K, K), f.slabs_a);
+    if (f.pair) {
+        hipLaunchKernelGGL(linear_pair_kernel, dim3((unsigned)(f.pw.blocks() + f.pa.blocks())), dim3(256), 0, s, pw, pa, (int)f.pw.blocks());
+        launch_join(pw, mode, s);
+        launch_join(pa, OUT_BF16, s);
+        return pdt_launch_status();
+    }
+    if (da) launch_gemm<false, true>(f.pa, pa, OUT_BF16, s);
+    launch_gemm<true, true>(f.pw, pw, mode, s);
     return pdt_launch_status();
 }

@@ -99,13 +99,12 @@ _sig("pdt_bnfold_sums", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp)
 _sig("pdt_distill_ce", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _i, _i, _f, _f,
      _f, _vp)
 _sig("pdt_top_logits", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _f, _vp)
-_sig("pdt_linear_fwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i, _i, _vp)
-_sig("pdt_linear_da", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _vp)
-_sig("pdt_linear_dw", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _vp)
-_sig("pdt_linear_dz", _vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _i, _i, _i, _vp)
-_sig("pdt_linear_pack", _vp, _vp, _ll, _i, _i, _i, _vp)
-_sig("pdt_linear_workspace", _ll, _ll, _ll)
-_real.pdt_linear_workspace.restype = _ll
+_sig("pdt_linear_fwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i, _vp)
+_sig("pdt_linear_bwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _vp)
+_sig("pdt_linear_fwd_workspace", _vp, _vp, _i, _i, _i, _ll, _ll)
+_sig("pdt_linear_bwd_workspace", _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i)
+_real.pdt_linear_fwd_workspace.restype = _ll
+_real.pdt_linear_bwd_workspace.restype = _ll
 _sig("pdt_set_deterministic", _i)
 _sig("pdt_accumulator_rows")
 
@@ -180,11 +179,11 @@ def _check(rc: int, what: str) -> None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _stream() -> int:
+def _stream(device: Optional[int] = None) -> int:
     # hundreds of launches per step: the raw-handle query is ~10x cheaper than building a
     # torch.cuda.Stream object each time
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device() if device is None else device)
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -1279,30 +1278,6 @@ def ce_metrics(logits, labels):
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
-def _few_rows(M: int, N: int, K: int) -> bool:
-    """Whether a forward product goes to the kernel for few rows, which reads ``a`` once per 16 rows of ``w``: 4096 x 4096 with
-    32 rows 14.6 us against 15.5 with tiles, with 64 rows 23.1 / 16.8; 16384 x 4096 with 4 rows 31.9 / 37.9, with 16 rows
-    40.0 / 38.2.  Where K is no multiple of 8 tiles need padded copies first: 6 us more at 777 x 1021, 13.2 us with 64 rows."""
-    return M <= 64 and M * N * K <= (1 << 29 if K % 8 == 0 else 1 << 31)
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with rows that start and end at 16-byte boundaries (zeros behind the last column), as the tile kernel's staging
-    needs them: ``t`` itself, or a copy."""
-    rows, cols = t.shape
-    ld = t.stride(0)
-    if cols % 8 == 0 and ld % 8 == 0 and cols <= ld < 1 << 22 and t.data_ptr() % 16 == 0:
-        return t
-    out = torch.empty(rows, (cols + 7) // 8 * 8, dtype=t.dtype, device=t.device)
-    _check(_lib.pdt_linear_pack(t.data_ptr(), out.data_ptr(), ld, out.shape[1], rows, cols, _stream()), "pdt_linear_pack")
-    return out
-
-
-def _linear_workspace(M: int, N: int, K: int, device) -> Optional[torch.Tensor]:
-    floats = _real.pdt_linear_workspace(M, N, K)
-    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
-
-
 def linear_act_fwd(a, w, bias=None, act: str = "none", residual=None, save: bool = False):
     # (a single row takes the GPU 5 us: the usual case is recognised by one expression, the others by the full check)
     sa, sw = a.shape, w.shape
@@ -1316,15 +1291,12 @@ def linear_act_fwd(a, w, bias=None, act: str = "none", residual=None, save: bool
     dev = a.device
     y = torch.empty(M, ld, dtype=_BF16, device=dev)
     z = torch.empty(M, ld, dtype=_BF16, device=dev) if save and act != "none" else None
-    few, ws = _few_rows(M, N, K), None
-    if not few:
-        a, w = _rows16(a), _rows16(w)
-        K = (K + 7) // 8 * 8
-        ws = _linear_workspace(M, N, K, dev)
-    rc = _lib.pdt_linear_fwd(a.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(),
-                             None if residual is None else residual.data_ptr(), y.data_ptr(), None if z is None else z.data_ptr(),
-                             None if ws is None else ws.data_ptr(), M, N, K, a.stride(0), w.stride(0),
-                             0 if residual is None else residual.stride(0), ld, LINEAR_ACTS[act], few, _raw_stream(cur))
+    ap, wp, lda, ldw = a.data_ptr(), w.data_ptr(), a.stride(0), w.stride(0)
+    need = _real.pdt_linear_fwd_workspace(ap, wp, M, N, K, lda, ldw)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = _lib.pdt_linear_fwd(ap, wp, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                             y.data_ptr(), None if z is None else z.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, lda,
+                             ldw, 0 if residual is None else residual.stride(0), ld, LINEAR_ACTS[act], _stream(cur))
     if rc:
         _check(rc, "pdt_linear_fwd")
     if ld != N:
@@ -1335,35 +1307,24 @@ def linear_act_fwd(a, w, bias=None, act: str = "none", residual=None, save: bool
 
 def linear_act_bwd(a, w, dy, z=None, act: str = "none", dw=None, dbias=None, need_da: bool = True):
     check_linear_act_bwd(a, w, dy, z, act, dw, dbias)
-    _here("linear_act_bwd", a, w, dy, z, dw, dbias)
+    cur = _here("linear_act_bwd", a, w, dy, z, dw, dbias)
     M, K = a.shape
-    N, dev, st = w.shape[0], a.device, _stream()
-    da = torch.empty(M, K, dtype=torch.bfloat16, device=dev) if need_da else None
+    N, dev, code = w.shape[0], a.device, LINEAR_ACTS[act]
+    da = torch.empty(M, K, dtype=_BF16, device=dev) if need_da else None
     add_w, add_b = dw is not None, dbias is not None
     if M == 0:
-        return (da, dw if add_w else torch.zeros(N, K, dtype=torch.bfloat16, device=dev),
-                dbias if add_b else torch.zeros(N, dtype=torch.float32, device=dev))
-    dw = dw if add_w else torch.empty(N, K, dtype=torch.bfloat16, device=dev)
-    dbias = dbias if add_b else torch.empty(N, dtype=torch.float32, device=dev)
-    # dy itself is the products' operand where there is no slope and its rows are aligned; else a padded bf16 dz
-    as_is = act == "none" and N % 8 == 0 and dy.stride(0) % 8 == 0 and N <= dy.stride(0) < 1 << 22 and dy.data_ptr() % 16 == 0
-    dz = dy if as_is else torch.empty(M, _npad(N), dtype=torch.bfloat16, device=dev)
-    # row blocks: about four workgroups per CU, each with at least 32 rows
-    parts = max(1, min((M + 31) // 32, 1024 * 256 // _npad(N)))
-    ws = torch.empty(parts * N, dtype=torch.float32, device=dev) if parts > 1 else None
-    rc = _lib.pdt_linear_dz(dy.data_ptr(), _p(z) if act != "none" else None, None if as_is else dz.data_ptr(), dbias.data_ptr(), _p(ws),
-                            M, N, dy.stride(0), z.stride(0) if z is not None else 0, dz.stride(0), LINEAR_ACTS[act], parts,
-                            int(add_b), st)
-    _check(rc, "pdt_linear_dz")
-    if need_da:
-        w16 = _rows16(w)
-        ws = _linear_workspace(M, K, (N + 7) // 8 * 8, dev)
-        _check(_lib.pdt_linear_da(dz.data_ptr(), w16.data_ptr(), da.data_ptr(), _p(ws), M, N, K, dz.stride(0), w16.stride(0), K, st),
-               "pdt_linear_da")
-    a16 = _rows16(a)
-    ws = _linear_workspace(N, K, M, dev)
-    _check(_lib.pdt_linear_dw(dz.data_ptr(), a16.data_ptr(), dw.data_ptr(), _p(ws), M, N, K, dz.stride(0), a16.stride(0),
-                              dw.stride(0), int(add_w), st), "pdt_linear_dw")
+        return (da, dw if add_w else torch.zeros(N, K, dtype=_BF16, device=dev),
+                dbias if add_b else torch.zeros(N, dtype=_F32, device=dev))
+    dw = dw if add_w else torch.empty(N, K, dtype=_BF16, device=dev)
+    dbias = dbias if add_b else torch.empty(N, dtype=_F32, device=dev)
+    yp, ap, wp, ldy, lda, ldw = dy.data_ptr(), a.data_ptr(), w.data_ptr(), dy.stride(0), a.stride(0), w.stride(0)
+    need = _real.pdt_linear_bwd_workspace(yp, ap, wp, M, N, K, ldy, lda, ldw, code, need_da)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = _lib.pdt_linear_bwd(yp, z.data_ptr() if code else None, ap, wp, None if da is None else da.data_ptr(), dw.data_ptr(),
+                             dbias.data_ptr(), None if ws is None else ws.data_ptr(), M, N, K, ldy, z.stride(0) if code else 0, lda, ldw,
+                             max(dw.stride(0), K), code, add_w, add_b, _stream(cur))    # (a lone row's stride says nothing)
+    if rc:
+        _check(rc, "pdt_linear_bwd")
     return da, dw, dbias
 
 
@@ -1389,7 +1350,7 @@ def top_logits(logits, k: int, temperature: float = 1.0):
     indices = torch.empty(B, k, dtype=torch.int32, device=dev)
     lse = torch.empty(B, dtype=_F32, device=dev)
     rc = _lib.pdt_top_logits(logits.data_ptr(), values.data_ptr(), indices.data_ptr(), lse.data_ptr(), B, N, k, logits.stride(0),
-                             _LOGIT_TYPES[dtype], temperature, _raw_stream(cur))
+                             _LOGIT_TYPES[dtype], temperature, _stream(cur))
     if rc:
         _check(rc, "pdt_top_logits")
     return values, indices, lse
@@ -1408,7 +1369,7 @@ def distill_ce(logits, labels, values, indices, temperature: float = 1.0, alpha:
                              None if lse is None else lse.data_ptr(), dlog.data_ptr(), at + 4, at, B, N, values.shape[1],
                              logits.stride(0), ld_val, st_val, ld_idx, st_idx, ld_out, _LOGIT_TYPES[dtype],
                              _LOGIT_TYPES[values.dtype], 8 if labels is None else labels.element_size(), indices.element_size(),
-                             temperature, alpha, grad_scale, _raw_stream(cur))
+                             temperature, alpha, grad_scale, _stream(cur))
     if rc:
         _check(rc, "pdt_distill_ce")
     return losses[0], dlog if ld_out == N else torch.as_strided(dlog, (B, N), (ld_out, 1))

@@ -134,6 +134,22 @@ def test_no_rows(hip, device):
     assert (buf == 1).all() and (vec == 1).all()
 
 
+def test_single_rows_whose_stride_says_nothing(hip, device):
+    """[1, K] views may have any stride between their (no) rows."""
+    gen = torch.Generator().manual_seed(8)
+    K, N = 72, 40
+    lone = [oracle.rows((1, n), gen, device=device).as_strided((1, n), (s, 1)) for n, s in ((K, 1), (N, 3), (K, 0), (1, 5))]
+    a, dy, w1, dy1 = lone
+    w = oracle.rows((N, K), gen, device=device)
+    assert torch.equal(hip.linear_act_fwd(a, w)[0], hip.linear_act_fwd(a.clone().reshape(1, K), w)[0])
+    for got, want in zip(hip.linear_act_bwd(a, w, dy), hip.linear_act_bwd(a.reshape(K).clone()[None], w, dy.reshape(N).clone()[None])):
+        assert torch.equal(got, want)
+    buf = torch.ones(K, device=device).as_strided((1, K), (1, 1))
+    da, dw, db = hip.linear_act_bwd(a, w1, dy1, dw=buf)
+    assert dw is buf and torch.allclose(buf.double(), 1 + dy1.double() * a.double(), rtol=1e-6)
+    assert torch.allclose(da.double(), dy1.double() * w1.double(), rtol=2.0 ** -8) and float(db) == float(dy1)
+
+
 def test_beyond_two_gigabytes(hip, device):
     """Offsets of operands and results pass 32 bits: the last rows against the same rows alone."""
     gen = torch.Generator().manual_seed(2)
@@ -180,21 +196,23 @@ def test_refusals(hip, device):
     with pytest.raises(ValueError):
         hip.linear_act_bwd(a, w, torch.zeros(6, 4, device=device).bfloat16(), act="gelu")
     fn, n = hip._real.pdt_linear_fwd, None
-    good = [n] * 7 + [0, 4, 8, 8, 8, 0, 64, 0, 0, n]
+    good = [n] * 7 + [0, 4, 8, 8, 8, 0, 64, 0, n]
     assert fn(*good) == 0
-    for at, bad in ((7, -1), (8, 0), (9, 0), (13, 3), (13, 63), (14, 4), (14, -1)):
+    for at, bad in ((7, -1), (8, 0), (9, 0), (13, 3), (13, 63), (13, 128), (14, 4), (14, -1)):
         args = list(good)
         args[at] = bad
         assert fn(*args) == -1, (at, bad)
-    args = list(good)
-    args[7], args[10], args[11] = 100, 8, 8
-    for at, bad in ((10, 7), (9, 7), (0, 2), (11, 1 << 22)):   # rows that are not aligned, K that is not padded
-        other = list(args)
-        other[at] = bad
-        assert fn(*other) == -2, (at, bad)
-    few = list(good)
-    few[7], few[15] = 65, 1
-    assert fn(*few) == -1
+    many = list(good)
+    many[7], many[9], many[10], many[11] = 100, 7, 7, 7         # copies of both operands, and no workspace for them
+    assert fn(*many) == -3
+    assert hip._real.pdt_linear_fwd_workspace(n, n, 100, 4, 7, 7, 7) >= 104 * 16
+    fn = hip._real.pdt_linear_bwd
+    good = [n] * 8 + [6, 4, 7, 4, 4, 7, 7, 7, 0, 0, 0, n]
+    assert fn(*good) == -3
+    for at, bad in ((8, 0), (9, 0), (10, 0), (15, 6), (16, 4), (16, -1), (16, 2)):   # (an activation without z)
+        args = list(good)
+        args[at] = bad
+        assert fn(*args) == -1, (at, bad)
 
 
 # ------------------------------------------------------------------------------------------------ a head that is distilled
