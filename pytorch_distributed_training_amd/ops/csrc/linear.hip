@@ -449,12 +449,39 @@ __global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_
     gemm_tile<BM, BN, RING, AT, BT>(p, blockIdx.x, smem);
 }
 
-// Both gradients of a layer in one launch: dw = dz^T a in the first workgroups, da = dz w in the rest.  Where neither has
+struct SumsJob {
+    const float* part;
+    float* out;
+    int N, parts, add, blocks;
+};
+// 64 columns a block, its four waves share the parts; the waves' sums are added in order
+__device__ __forceinline__ void join_sums(const SumsJob& p, int block, float (*red)[64]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = block * 64 + lane;
+    float t = 0.0f;
+    if (c < p.N) {
+#pragma unroll 8
+        for (int i = wave; i < p.parts; i += 4) t += p.part[(long long)i * p.N + c];
+    }
+    red[wave][lane] = t;
+    __syncthreads();
+    if (wave == 0 && c < p.N) {
+        t = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+        p.out[c] = p.add ? p.out[c] + t : t;
+    }
+}
+__global__ __launch_bounds__(256) void linear_sums_kernel(const SumsJob p) {
+    __shared__ float red[4][64];
+    join_sums(p, blockIdx.x, red);
+}
+
+// Both gradients of a layer in one launch: dw = dz^T a in the first workgroups, da = dz w in the next, dbias in the last.  Where neither has
 // tiles enough for the chip, each alone would leave CUs idle or pay for a split of its K.
-__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int first) {
+__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int first, int second,
+                                                             const SumsJob sums) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[5 * 128 * LIN_BK * 2];
     if ((int)blockIdx.x < first) gemm_tile<128, 128, 5, true, true>(dw, blockIdx.x, smem);
-    else gemm_tile<128, 128, 5, false, true>(da, blockIdx.x - first, smem);
+    else if ((int)blockIdx.x < first + second) gemm_tile<128, 128, 5, false, true>(da, blockIdx.x - first, smem);
+    else join_sums(sums, blockIdx.x - first - second, reinterpret_cast<float(*)[64]>(smem));
 }
 
 // Joins the partial sums of a product whose K range was split (too few tiles for the chip), in slab order, and does what the
@@ -598,23 +625,6 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const bf16* __restrict__
     float* out = sums + (long long)blockIdx.y * N + c;
     *out = add ? *out + t : t;
 }
-// 64 columns a block, its four waves share the parts; the waves' sums are added in order
-__global__ __launch_bounds__(256) void linear_sums_kernel(const float* __restrict__ part, float* __restrict__ out, int N,
-                                                          int parts, int add) {
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    float t = 0.0f;
-    if (c < N) {
-#pragma unroll 8
-        for (int i = wave; i < parts; i += 4) t += part[(long long)i * N + c];
-    }
-    red[wave][lane] = t;
-    __syncthreads();
-    if (wave == 0 && c < N) {
-        t = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
-        out[c] = add ? out[c] + t : t;
-    }
-}
 
 // rows of any stride and alignment -> rows of ldp columns (a multiple of 8), zeros behind the last one; one or two matrices
 struct PackJob {
@@ -685,7 +695,7 @@ static Plan plan_of(long long M, long long N, long long K) {
 
 // Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then.  Two workgroups on a CU take
 // 0.75 us a step where the chip is not full, and the same 0.43 us per tile and CU where it is; a launch of its own costs about
-// 2 us.  1536 x 2048 x 1000: PAIR_US us against SOLO_US.
+// 2 us.  1536 x 2048 x 1000: 33.6 us with dbias against 44.1 (30.9 with the column sums in the same launch).
 static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da) {
     dw = plan_of(N, K, M), da = plan_of(M, K, N);
     const long long tw = (long long)cdiv(N, 128) * cdiv(K, 128), ta = (long long)cdiv(M, 128) * cdiv(K, 128);
@@ -903,15 +913,16 @@ PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const v
                        act == LIN_NONE ? nullptr : static_cast<const bf16*>(z), f.dz_out,
                        f.n_parts > 1 ? f.parts : static_cast<float*>(dbias), lddy, ldz, (int)f.dz.ld, M, N, act, cdiv(M, f.n_parts),
                        f.n_parts > 1 ? 0 : add_b);
-    if (f.n_parts > 1)
-        hipLaunchKernelGGL(linear_sums_kernel, dim3(cdiv(N, 64)), dim3(256), 0, s, f.parts, static_cast<float*>(dbias), N, f.n_parts, add_b);
+    const SumsJob sums = {f.parts, static_cast<float*>(dbias), N, f.n_parts, add_b, f.n_parts > 1 ? cdiv(N, 64) : 0};
+    if (sums.blocks > 0 && !f.pair) hipLaunchKernelGGL(linear_sums_kernel, dim3(sums.blocks), dim3(256), 0, s, sums);
     launch_pack(f.ja, f.jw, s);
     const int mode = add_w ? OUT_ADD : OUT_BF16;
     const GemmParams pw = gemm_params(f.pw, f.dz, f.a, M, plain_epilogue(dw, mode, N, K, lddw), f.slabs_w);
     GemmParams pa;
     if (da) pa = gemm_params(f.pa, f.dz, f.w, pad8(N), plain_epilogue(da, OUT_BF16, M, K, K), f.slabs_a);
     if (f.pair) {
-        hipLaunchKernelGGL(linear_pair_kernel, dim3((unsigned)(f.pw.blocks() + f.pa.blocks())), dim3(256), 0, s, pw, pa, (int)f.pw.blocks());
+        const int first = (int)f.pw.blocks(), second = (int)f.pa.blocks();
+        hipLaunchKernelGGL(linear_pair_kernel, dim3(first + second + sums.blocks), dim3(256), 0, s, pw, pa, first, second, sums);
         launch_join(pw, mode, s);
         launch_join(pa, OUT_BF16, s);
         return pdt_launch_status();
