@@ -474,14 +474,15 @@ __global__ __launch_bounds__(256) void linear_sums_kernel(const SumsJob p) {
     join_sums(p, blockIdx.x, red);
 }
 
-// Both gradients of a layer in one launch: dw = dz^T a in the first workgroups, da = dz w in the next, dbias in the last.  Where neither has
+// Both gradients of a layer in one launch, dw = dz^T a and da = dz w, that with more steps first, and dbias in the last blocks.  Where neither has
 // tiles enough for the chip, each alone would leave CUs idle or pay for a split of its K.
-__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int first, int second,
-                                                             const SumsJob sums) {
+__global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int dw_at, int da_at,
+                                                             int sums_at, const SumsJob sums) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[5 * 128 * LIN_BK * 2];
-    if ((int)blockIdx.x < first) gemm_tile<128, 128, 5, true, true>(dw, blockIdx.x, smem);
-    else if ((int)blockIdx.x < first + second) gemm_tile<128, 128, 5, false, true>(da, blockIdx.x - first, smem);
-    else join_sums(sums, blockIdx.x - first - second, reinterpret_cast<float(*)[64]>(smem));
+    const int block = blockIdx.x;
+    if (block >= sums_at) join_sums(sums, block - sums_at, reinterpret_cast<float(*)[64]>(smem));
+    else if (block >= dw_at && (dw_at > da_at || block < da_at)) gemm_tile<128, 128, 5, true, true>(dw, block - dw_at, smem);
+    else gemm_tile<128, 128, 5, false, true>(da, block - da_at, smem);
 }
 
 // Joins the partial sums of a product whose K range was split (too few tiles for the chip), in slab order, and does what the
@@ -494,6 +495,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const Epilogue p, int 
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < p.N) {
         const float* slab = p.ws + m * slab_ld(p.N) + n;
+#pragma unroll 8
         for (int s = 0; s < splits; ++s, slab += p.M * slab_ld(p.N)) {
             const f32x4 lo = *reinterpret_cast<const f32x4*>(slab), hi = *reinterpret_cast<const f32x4*>(slab + 4);
 #pragma unroll
@@ -516,8 +518,9 @@ template <int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(const bf16* __restrict__ a, const bf16* __restrict__ w,
                                                               long long lda, long long ldw, int K, const Epilogue ep) {
     __shared__ f32x4 part[NW][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int x = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // matrix instructions run under any exec mask: branches
+    const int x = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;        // around them have to be scalar
     const bf16* wr = w + (long long)min(n0 + x, ep.N - 1) * ldw;       // rows past the end: computed and dropped
     const bf16* ar[MT];
 #pragma unroll
@@ -526,10 +529,12 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(const bf16* __rest
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto load = [&](const bf16* p, int k) -> bf16x8 { return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_a2*>(p + k)); };
-    constexpr int U = 4;                                               // fragments of w a wave has in flight
+    // U fragments of w at a time, the next U on their way while these are multiplied
+    constexpr int U = 4;
     const int steps = K / 32;
-    for (int r = wave * U; r < steps; r += NW * U) {
-        bf16x8 wf[U], af[MT][U];
+    bf16x8 w0[U], a0[MT][U], w1[U], a1[MT][U];
+    auto fetch = [&](bf16x8 (&wf)[U], bf16x8 (&af)[MT][U], int r) {
+        if (r >= steps) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = min(r + u, steps - 1) * 32 + g * 8;          // past the last step: loaded again, not multiplied
@@ -537,12 +542,22 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(const bf16* __rest
 #pragma unroll
             for (int t = 0; t < MT; ++t) af[t][u] = load(ar[t], k);
         }
+    };
+    auto multiply = [&](const bf16x8 (&wf)[U], const bf16x8 (&af)[MT][U], int r) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (r + u < steps) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[u], af[t][u], acc[t], 0, 0, 0);
             }
+    };
+    int r = wave * U;
+    fetch(w0, a0, r);
+    for (; r < steps; r += 2 * NW * U) {
+        fetch(w1, a1, r + NW * U);
+        multiply(w0, a0, r);
+        fetch(w0, a0, r + 2 * NW * U);
+        multiply(w1, a1, r + NW * U);
     }
     if (wave == NW - 1 && steps * 32 < K) {                            // the last, partial step
         const int k = steps * 32 + g * 8;
@@ -667,8 +682,10 @@ static void cut(Plan& q, int tile, long long M, long long N, int nk, int splits)
     q.big = tile == 256, q.tiles_m = cdiv(M, tile), q.tiles_n = cdiv(N, tile);
     q.steps = cdiv(nk, splits), q.splits = cdiv(nk, q.steps);
 }
-// joining partial sums: 4 us and their way through memory at 4.5 TB/s
-static long long join_cost(long long M, long long N, int splits) { return splits > 1 ? 400 + splits * M * N * 8 / 45000 : 0; }
+// joining partial sums: 4 us, 0.08 us a slab and their way through memory at 4.5 TB/s
+static long long join_cost(long long M, long long N, int splits) {
+    return splits > 1 ? 400 + splits * 8 + splits * M * N * 8 / 45000 : 0;
+}
 
 static Plan plan_of(long long M, long long N, long long K) {
     Plan q;
@@ -796,11 +813,20 @@ static Epilogue plain_epilogue(void* out, int mode, int M, int N, long long ldo)
     return e;
 }
 
-// Whether a forward product goes to the kernel for few rows, which reads a once per 16 rows of w: 4096 x 4096 with 32 rows
-// 14.6 us against 15.5 with tiles, with 64 rows 23.1 / 16.8; 16384 x 4096 with 4 rows 31.9 / 37.9, with 16 rows 40.0 / 38.2.
-// Rows that tiles need copied first (777 x 1021: 6 us more) leave it ahead for longer.
-static bool few_rows(int M, int N, int K, bool copies) {
-    return M <= 64 && (long long)M * N * K <= (copies ? 1ll << 31 : 1ll << 29);
+// Whether a forward product goes to the kernel for few rows.  It reads w at 4.9 TB/s and, once for every 16 rows of w, a out of
+// the caches at 7 TB/s; where there is little of both, 1024 columns of K take a wave 0.9 us and 0.05 us per row of a.  Tiles
+// are bound by w's way through memory at least, and pay for copies of what is not laid out for them.  Measured, few rows / tiles:
+// 4096 x 4096 with 1 row 8.3 / 14.0 us, with 64 rows 21.4 / 15.9; 16384 x 4096 with 4 rows 26 / 38, with 32 rows 54 / 39;
+// 276 x 7928 with 4 rows 10.1 / 15.7, with 64 rows 30 / 15.7; 777 x 1021 with 16 rows 6.4 / 12.5.
+static bool few_rows(const Matrix& a, const Matrix& w, const Plan& tiles) {
+    if (a.rows > 64) return false;
+    const long long M = a.rows, N = w.rows, K = a.cols;
+    const long long trips = cdiv(K, 1024) * (90 + 5 * M) + 220, bytes = N * K * 2 / 49000 + M * K * 2 * cdiv(N, 16) / 70000;
+    long long copies = 0;
+    if (!a.fits()) copies += M * K * 4;
+    if (!w.fits()) copies += N * K * 4;
+    const long long floor = 500 + N * K * 2 / 49000, cost = (tiles.cost > floor ? tiles.cost : floor) + 150;
+    return (trips > bytes ? trips : bytes) < cost + (copies > 0 ? 250 + copies / 49000 : 0);
 }
 struct FwdPlan {
     Matrix a, w;
@@ -813,12 +839,12 @@ struct FwdPlan {
 static FwdPlan plan_fwd(const void* a, const void* w, void* ws, int M, int N, int K, long long lda, long long ldw) {
     FwdPlan f;
     f.a = Matrix{static_cast<const bf16*>(a), lda, M, K}, f.w = Matrix{static_cast<const bf16*>(w), ldw, N, K};
-    f.few = few_rows(M, N, K, !f.a.fits() || !f.w.fits());
+    f.plan = plan_of(M, N, pad8(K));
+    f.few = few_rows(f.a, f.w, f.plan);
     f.slabs = nullptr, f.ja.blocks = f.jw.blocks = 0;
     Arena mem{static_cast<unsigned char*>(ws)};
     if (!f.few) {
         f.a = operand(f.a, mem, f.ja), f.w = operand(f.w, mem, f.jw);
-        f.plan = plan_of(M, N, pad8(K));
         f.slabs = static_cast<float*>(mem.take(slab_bytes(f.plan, M, N)));
     }
     f.bytes = mem.used;
@@ -921,8 +947,10 @@ PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const v
     GemmParams pa;
     if (da) pa = gemm_params(f.pa, f.dz, f.w, pad8(N), plain_epilogue(da, OUT_BF16, M, K, K), f.slabs_a);
     if (f.pair) {
-        const int first = (int)f.pw.blocks(), second = (int)f.pa.blocks();
-        hipLaunchKernelGGL(linear_pair_kernel, dim3(first + second + sums.blocks), dim3(256), 0, s, pw, pa, first, second, sums);
+        const int nw = (int)f.pw.blocks(), na = (int)f.pa.blocks();
+        const bool da_first = f.pa.steps > f.pw.steps;
+        hipLaunchKernelGGL(linear_pair_kernel, dim3(nw + na + sums.blocks), dim3(256), 0, s, pw, pa, da_first ? na : 0,
+                           da_first ? 0 : nw, nw + na, sums);
         launch_join(pw, mode, s);
         launch_join(pa, OUT_BF16, s);
         return pdt_launch_status();

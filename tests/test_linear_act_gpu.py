@@ -52,6 +52,36 @@ def test_forward(hip, device, act, M, N, K):
             padding_is_zero(z, N)
 
 
+@pytest.mark.parametrize("M", [1, 5, 16, 17, 32, 33, 64])
+def test_few_rows_of_many_lengths(hip, device, M):
+    """Waves with no, one, an odd number and a partial turn of K."""
+    gen = torch.Generator().manual_seed(M)
+    for K in (8, 31, 32, 40, 127, 128, 256, 288, 1024, 1056, 1216, 2040, 2176, 3200, 4608):
+        for N in (10, 100, 300):
+            a, w = oracle.rows((M, K), gen, device=device), oracle.rows((N, K), gen, scale=K ** -0.5, device=device)
+            y, _ = hip.linear_act_fwd(a, w)
+            want, _, bound, _ = oracle.fwd(a, w, None, "none", None)
+            within(y, want, bound)
+
+
+@pytest.mark.parametrize("M,N,K", [(64, 30, 4000), (2000, 40, 60), (40, 3000, 50), (700, 2100, 1900), (2200, 2304, 2100), (60, 5000, 5000)])
+def test_gradients_in_one_launch_and_apart(hip, device, M, N, K):
+    gen = torch.Generator().manual_seed(N)
+    a, w = oracle.rows((M, K), gen, device=device), oracle.rows((N, K), gen, scale=K ** -0.5, device=device)
+    dy = oracle.rows((M, N), gen, device=device)
+    want, bounds = oracle.bwd(a, w, dy, None, "none")
+    for need_da in (True, False):
+        got = hip.linear_act_bwd(a, w, dy, need_da=need_da)
+        assert (got[0] is None) == (not need_da)
+        for g, x, b in zip(got, want, bounds):
+            if g is not None:
+                within(g, x, b)
+        buf, vec = torch.full((N, K), 7.0, device=device), torch.full((N,), 3.0, device=device)
+        hip.linear_act_bwd(a, w, dy, dw=buf, dbias=vec, need_da=need_da)
+        within(buf - 7.0, want[1], bounds[1] + 2.0 ** -21 + 2.0 ** -23 * want[1].abs())
+        within(vec - 3.0, want[2], bounds[2] + 2.0 ** -22 + 2.0 ** -23 * want[2].abs())
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_backward(hip, device, act, M, N, K):
