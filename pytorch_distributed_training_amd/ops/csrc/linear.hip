@@ -474,8 +474,8 @@ __global__ __launch_bounds__(256) void linear_sums_kernel(const SumsJob p) {
     join_sums(p, blockIdx.x, red);
 }
 
-// Both gradients of a layer in one launch, dw = dz^T a and da = dz w, that with more steps first, and dbias in the last blocks.  Where neither has
-// tiles enough for the chip, each alone would leave CUs idle or pay for a split of its K.
+// Both gradients of a layer in one launch, dw = dz^T a and da = dz w, that with more steps first, and dbias in the last
+// blocks.  Each alone would leave CUs idle, at its end at least, or pay for a split of its K.
 __global__ __launch_bounds__(256, 2) void linear_pair_kernel(const GemmParams dw, const GemmParams da, int dw_at, int da_at,
                                                              int sums_at, const SumsJob sums) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[5 * 128 * LIN_BK * 2];
@@ -710,16 +710,17 @@ static Plan plan_of(long long M, long long N, long long K) {
     return q;
 }
 
-// Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then.  Two workgroups on a CU take
-// 0.75 us a step where the chip is not full, and the same 0.43 us per tile and CU where it is; a launch of its own costs about
-// 2 us.  1536 x 2048 x 1000: 33.6 us with dbias against 44.1 (30.9 with the column sums in the same launch).
+// Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then: where neither takes the large
+// tiles.  Two workgroups on a CU take 0.75 us a step where the chip is not full, and 0.43 us per tile and CU where it is.
+// One launch / two, with dbias: 1536 x 1000 x 2048 28.4 / 44.0 us, 64 x 4096 x 4096 30.9 / 37.1, 1024 x 4096 x 4096 83.7 / 94.7,
+// 300 x 16384 x 4096 147 / 163; where one takes large tiles 2048 x 4096 x 4096 142 / 144, where both do 4096 x 4096 x 4096 279 / 242.
 static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da) {
     dw = plan_of(N, K, M), da = plan_of(M, K, N);
+    if (dw.big || da.big) return false;
     const long long tw = (long long)cdiv(N, 128) * cdiv(K, 128), ta = (long long)cdiv(M, 128) * cdiv(K, 128);
     const int nw = cdiv(M, LIN_BK), na = cdiv(N, LIN_BK);
-    if (tw + ta > 8 * LIN_CUS) return false;                   // each fills the chip
-    long long best = dw.cost + da.cost + 200;
-    int best_w = 0, best_a = 0;
+    long long best = -1;
+    int best_w = 1, best_a = 1;
     for (int sw = 1; sw == 1 || (sw <= 16 && sw <= nw / 2 && sw * tw <= 2 * LIN_CUS); ++sw)
         for (int sa = 1; sa == 1 || (sa <= 16 && sa <= na / 2 && sa * ta <= 2 * LIN_CUS); ++sa) {
             const int kw = cdiv(nw, sw), ka = cdiv(na, sa), k = kw > ka ? kw : ka;
@@ -728,9 +729,8 @@ static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da)
             const long long one = 275 + (blocks <= LIN_CUS ? 56ll : 75ll) * k, rounds = blocks > 2 * LIN_CUS ? work + one / 2 : 0;
             long long cost = work > one ? work : one;
             cost = (cost > rounds ? cost : rounds) + join_cost(N, K, sw) + join_cost(M, K, sa);
-            if (cost < best) best = cost, best_w = sw, best_a = sa;
+            if (best < 0 || cost < best) best = cost, best_w = sw, best_a = sa;
         }
-    if (!best_w) return false;
     cut(dw, 128, N, K, nw, best_w), cut(da, 128, M, K, na, best_a);
     return true;
 }
@@ -932,7 +932,7 @@ PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const v
                            int add_w, int add_b, hipStream_t s) {
     if (M < 1 || N < 1 || K < 1 || lddw < K || lddw > 0x7fffffffll || act < 0 || act > LIN_SILU || (act != LIN_NONE && !z)) return -1;
     const BwdPlan f = plan_bwd(dy, a, w, ws, M, N, K, lddy, lda, ldw, act, da != nullptr);
-    if (f.pw.blocks() > 0x7fffffffll || (da && f.pa.blocks() > 0x7fffffffll)) return -1;
+    if (f.pw.blocks() + (da ? f.pa.blocks() : 0) + N > 0x7fffffffll) return -1;
     if (f.bytes > 0 && !ws) return -3;
     const int cols = f.dz_out ? pad64(N) : N;
     hipLaunchKernelGGL(linear_dz_kernel, dim3(cdiv(cols, 256), f.n_parts), dim3(256), 0, s, static_cast<const bf16*>(dy),
