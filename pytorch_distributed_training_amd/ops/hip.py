@@ -1362,17 +1362,18 @@ def distill_ce(logits, labels, values, indices, temperature: float = 1.0, alpha:
     cur = _here("distill_ce", logits, labels, values, indices, lse)
     (B, N), (ld_val, st_val), (ld_idx, st_idx) = logits.shape, values.stride(), indices.stride()
     ld_out, dev, dtype = (N + 63) // 64 * 64, logits.device, logits.dtype
-    dlog = torch.empty(B, ld_out, dtype=dtype, device=dev)
-    losses = torch.empty(B + 1, dtype=_F32, device=dev)               # the mean, then the rows' own
-    at = losses.data_ptr()
+    # the gradient and, behind it, the rows' own losses: one allocation (the call is bound by the host up to some 1500 x 1000)
+    buf = torch.empty(B * (ld_out + (1 if dtype is _F32 else 2)), dtype=dtype, device=dev)
+    loss = torch.empty((), dtype=_F32, device=dev)
+    at = buf.data_ptr()
     rc = _lib.pdt_distill_ce(logits.data_ptr(), None if labels is None else labels.data_ptr(), values.data_ptr(), indices.data_ptr(),
-                             None if lse is None else lse.data_ptr(), dlog.data_ptr(), at + 4, at, B, N, values.shape[1],
-                             logits.stride(0), ld_val, st_val, ld_idx, st_idx, ld_out, _LOGIT_TYPES[dtype],
+                             None if lse is None else lse.data_ptr(), at, at + B * ld_out * dtype.itemsize, loss.data_ptr(), B, N,
+                             values.shape[1], logits.stride(0), ld_val, st_val, ld_idx, st_idx, ld_out, _LOGIT_TYPES[dtype],
                              _LOGIT_TYPES[values.dtype], 8 if labels is None else labels.element_size(), indices.element_size(),
                              temperature, alpha, grad_scale, _stream(cur))
     if rc:
         _check(rc, "pdt_distill_ce")
-    return losses[0], dlog if ld_out == N else torch.as_strided(dlog, (B, N), (ld_out, 1))
+    return loss, torch.as_strided(buf, (B, N), (ld_out, 1))
 
 
 # --------------------------------------------------------------------------- optimizer
