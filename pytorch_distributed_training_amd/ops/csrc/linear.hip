@@ -274,11 +274,11 @@ struct Operand {
 template <int BM, int BN, int RING, bool AT, bool BT>
 __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, unsigned char* smem) {
     constexpr int WM = 2, WN = 2, NW = WM * WN, BK = LIN_BK, WTM = BM / WM, WTN = BN / WN, MI = WTM / 16, NI = WTN / 16;
-    static_assert(BM == BN && RING % 2 == 1 && RING >= 5, "slots of one size, filled in turn");
+    static_assert(RING % 2 == 1 && RING >= 5 && BM <= BN, "the slots are filled by a and b in turn");
     constexpr bool PERM = !BT;
     typedef Operand<AT, BM, NW, false> A;
     typedef Operand<BT, BN, NW, PERM> B;
-    constexpr int SLOT = A::BYTES, PER = A::PER;
+    constexpr int SLOT = B::BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -317,13 +317,16 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
     // n = 2 ks + RING (of b).  Reads and DMA go out between the products at an even pace: a wave has its SIMD to itself (or
     // shares it with one of another workgroup), so whatever is issued in a clump stops the matrix cores.  The stages past the
     // end of K are staged too, as zeros: no conditions, and the number of DMA in flight is a constant.
-    const unsigned wave_at = (unsigned)(unsigned long long)(lin_lds_void_t*)smem + wave * (PER * 1024);
+    const unsigned lds_at = (unsigned)(unsigned long long)(lin_lds_void_t*)smem;
+    const unsigned wave_a = lds_at + wave * (A::PER * 1024), wave_b = lds_at + wave * (B::PER * 1024);
     int rem_a = p.K - k0, rem_b = rem_a;                       // of K, from the stage that is staged next
     bf16x8 a0[MI], b0[NI], a1[MI], b1[NI];
-    constexpr int GROUPS = MI * NI / 4, READS = (MI + NI) / (GROUPS / 2), PACE = GROUPS / PER;
-    static_assert(READS * GROUPS / 2 == MI + NI && PACE * PER == GROUPS, "reads in the first half of the groups");
+    constexpr int GROUPS = MI * NI / 4, READS = (MI + NI) / (GROUPS / 2);
+    static_assert(READS * GROUPS / 2 == MI + NI, "reads in the first half of the groups");
     auto half = [&](const bf16x8 (&ac)[MI], const bf16x8 (&bc)[NI], bf16x8 (&an)[MI], bf16x8 (&bn)[NI], int sa, int sb, int kk,
-                    auto&& dma) {
+                    auto per, auto&& dma) {
+        constexpr int PER = decltype(per)::value, PACE = PER < GROUPS ? GROUPS / PER : 1, EACH = PER * PACE / GROUPS;
+        static_assert(EACH * GROUPS == PER * PACE, "DMA at an even pace");
         const unsigned char *as = smem + sa * SLOT, *bs = smem + sb * SLOT;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
@@ -334,7 +337,10 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
                     else an[(r - NI + MI) % MI] = A::read(as, wm * WTM, (r - NI + MI) % MI, kk, lane);
                 }
             }
-            if (g % PACE == 0) dma(g / PACE);
+            if (g % PACE == 0) {
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) dma(g / PACE * EACH + j);
+            }
 #pragma unroll
             for (int t = 4 * g; t < 4 * g + 4; ++t)            // (the compiler, left alone, moves half of the sums to VGPRs and spills)
                 asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[t / NI][t % NI]) : "v"(bc[t % NI]), "v"(ac[t / NI]));
@@ -343,17 +349,17 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
     };
     auto stage_a = [&](int slot) {
         const u32x4 d = a.desc();
-        unsigned m = wave_at + slot * SLOT;
+        unsigned m = wave_a + slot * SLOT;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) a.template piece<true>(d, m, rem_a, j, wave, lane);
+        for (int j = 0; j < A::PER; ++j) a.template piece<true>(d, m, rem_a, j, wave, lane);
         a.next();
         rem_a -= BK;
     };
     auto stage_b = [&](int slot) {
         const u32x4 d = b.desc();
-        unsigned m = wave_at + slot * SLOT;
+        unsigned m = wave_b + slot * SLOT;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) b.template piece<true>(d, m, rem_b, j, wave, lane);
+        for (int j = 0; j < B::PER; ++j) b.template piece<true>(d, m, rem_b, j, wave, lane);
         b.next();
         rem_b -= BK;
     };
@@ -362,7 +368,7 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
         stage_a(n);
         stage_b(n + 1);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 3) * PER) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 3) / 2 * (A::PER + B::PER)) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -375,18 +381,18 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
         constexpr bool TAIL = decltype(tail)::value;
         {
             const u32x4 d = a.desc();
-            unsigned m = wave_at + up(sa, RING - 1) * SLOT;
-            half(a0, b0, a1, b1, sa, up(sa, 1), 1, [&](int j) { a.template piece<TAIL>(d, m, rem_a, j, wave, lane); });
+            unsigned m = wave_a + up(sa, RING - 1) * SLOT;
+            half(a0, b0, a1, b1, sa, up(sa, 1), 1, std::integral_constant<int, A::PER>{}, [&](int j) { a.template piece<TAIL>(d, m, rem_a, j, wave, lane); });
             a.next();
             rem_a -= BK;
         }
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 4) * PER) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 3) / 2 * A::PER + (RING - 5) / 2 * B::PER) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         {
             const u32x4 d = b.desc();
-            unsigned m = wave_at + sa * SLOT;
-            half(a1, b1, a0, b0, up(sa, 2), up(sa, 3), 0, [&](int j) { b.template piece<TAIL>(d, m, rem_b, j, wave, lane); });
+            unsigned m = wave_b + sa * SLOT;
+            half(a1, b1, a0, b0, up(sa, 2), up(sa, 3), 0, std::integral_constant<int, B::PER>{}, [&](int j) { b.template piece<TAIL>(d, m, rem_b, j, wave, lane); });
             b.next();
             rem_b -= BK;
         }
@@ -444,8 +450,8 @@ __device__ __forceinline__ void gemm_tile(const GemmParams& p, const int block, 
 }
 
 template <int BM, int BN, int RING, bool AT, bool BT>
-__global__ __launch_bounds__(256, BM* RING <= 128 * 5 ? 2 : 1) void linear_gemm_kernel(const GemmParams p) {
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * BM * LIN_BK * 2];
+__global__ __launch_bounds__(256, BN* RING <= 128 * 5 ? 2 : 1) void linear_gemm_kernel(const GemmParams p) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[RING * BN * LIN_BK * 2];
     gemm_tile<BM, BN, RING, AT, BT>(p, blockIdx.x, smem);
 }
 
@@ -674,12 +680,12 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const PackJob j0, cons
 
 // How a product is cut up.  Costs are in units of 10 ns.
 struct Plan {
-    int big, splits, steps, tiles_m, tiles_n;
+    int rows, splits, steps, tiles_m, tiles_n;                   // rows of a tile: 256, 128 or 64
     long long cost;
     long long blocks() const { return (long long)tiles_m * tiles_n * splits; }
 };
-static void cut(Plan& q, int tile, long long M, long long N, int nk, int splits) {
-    q.big = tile == 256, q.tiles_m = cdiv(M, tile), q.tiles_n = cdiv(N, tile);
+static void cut(Plan& q, int rows, long long M, long long N, int nk, int splits) {
+    q.rows = rows, q.tiles_m = cdiv(M, rows), q.tiles_n = cdiv(N, rows == 256 ? 256 : 128);
     q.steps = cdiv(nk, splits), q.splits = cdiv(nk, q.steps);
 }
 // joining partial sums: 4 us, 0.08 us a slab and their way through memory at 4.5 TB/s
@@ -687,26 +693,36 @@ static long long join_cost(long long M, long long N, int splits) {
     return splits > 1 ? 400 + splits * 8 + splits * M * N * 8 / 45000 : 0;
 }
 
-static Plan plan_of(long long M, long long N, long long K) {
+// thin: 64 x 128 tiles are built for this product (the forward one)
+static Plan plan_of(long long M, long long N, long long K, bool thin) {
     Plan q;
     const int nk = cdiv(K, LIN_BK);
     // 256 x 256 tiles run one to a CU and take about 16 us plus 1.45 us a step of 64 each (most of the 16 us: nothing covers
     // their prologue and their 64 Ki results); 128 x 128 tiles run two to a CU and take 2.8 + 0.43 us per tile and CU.
     // 4096 x 16384 x 4096: 418 us against 580; x 1024: 156 / 152; x 128: 75 / 56; 2048 x 4096 x 4096 (128 tiles of 256): 91 / 63.
     const long long big = (long long)cdiv((long long)cdiv(M, 256) * cdiv(N, 256), LIN_CUS) * (1600 + 145ll * nk);
-    const long long tiles = (long long)cdiv(M, 128) * cdiv(N, 128), small = (long long)cdiv(tiles, LIN_CUS) * (275 + 43ll * nk);
-    q.cost = big < small ? big : small;
-    int splits = 1;
-    // K ranges, while one workgroup per CU holds them: a step of a lone 128 x 128 workgroup takes 0.56 us (1000 x 2048 x 1536,
+    // A lone 128 x 128 workgroup takes 0.56 us a step; K is split while one workgroup per CU holds the ranges (1000 x 2048 x 1536,
     // 128 tiles: one range 19 us, two 24; 64 x 4096 x 4096, 32 tiles: one 40 us, eight 16).
-    if (big >= small && tiles < LIN_CUS) {
-        q.cost = 275 + 56ll * nk;
+    const long long tiles = (long long)cdiv(M, 128) * cdiv(N, 128), two = (long long)cdiv(tiles, LIN_CUS) * (275 + 43ll * nk);
+    const long long lone = 275 + 56ll * nk, small = two > lone ? two : lone;
+    int rows = big < small ? 256 : 128, splits = 1;
+    q.cost = big < small ? big : small;
+    if (rows == 128) {
         for (int s = 2; s <= LIN_CUS / tiles && s <= nk / 2; ++s) {
             const long long cost = 275 + 56ll * cdiv(nk, s) + join_cost(M, N, s);
             if (cost < q.cost) q.cost = cost, splits = s;
         }
     }
-    cut(q, big < small ? 256 : 128, M, N, nk, splits);
+    // 64 x 128 tiles: 2.2 us and 0.34 us a step, no less with two on a CU.  Twice as many workgroups where there are few:
+    // 1536 x 1000 x 2048 16.0 us against 21.5 with 128 x 128, 128 x 4096 x 4096 15.6 / 18.2; 4096 x 4096 x 512 33.4 / 27.8.
+    if (thin && rows != 256) {
+        const long long t = (long long)cdiv(M, 64) * cdiv(N, 128), turns = cdiv(t, LIN_CUS);
+        for (int s = 1; s == 1 || (s <= LIN_CUS / t && s <= nk / 2); ++s) {
+            const long long cost = turns * (220 + 34ll * cdiv(nk, s)) + join_cost(M, N, s);
+            if (cost < q.cost) q.cost = cost, splits = s, rows = 64;
+        }
+    }
+    cut(q, rows, M, N, nk, splits);
     return q;
 }
 
@@ -715,8 +731,8 @@ static Plan plan_of(long long M, long long N, long long K) {
 // One launch / two, with dbias: 1536 x 1000 x 2048 28.4 / 44.0 us, 64 x 4096 x 4096 30.9 / 37.1, 1024 x 4096 x 4096 83.7 / 94.7,
 // 300 x 16384 x 4096 147 / 163; where one takes large tiles 2048 x 4096 x 4096 142 / 144, where both do 4096 x 4096 x 4096 279 / 242.
 static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da) {
-    dw = plan_of(N, K, M), da = plan_of(M, K, N);
-    if (dw.big || da.big) return false;
+    dw = plan_of(N, K, M, false), da = plan_of(M, K, N, false);
+    if (dw.rows == 256 || da.rows == 256) return false;
     const long long tw = (long long)cdiv(N, 128) * cdiv(K, 128), ta = (long long)cdiv(M, 128) * cdiv(K, 128);
     const int nw = cdiv(M, LIN_BK), na = cdiv(N, LIN_BK);
     long long best = -1;
@@ -799,7 +815,14 @@ template <bool AT, bool BT>
 static void launch_gemm(const Plan& q, const GemmParams& p, int mode, hipStream_t s) {
     const dim3 grid((unsigned)q.blocks());
     // 128 x 128 tiles: two workgroups of 80 KB on a CU where there are that many, else one with a deeper ring
-    if (q.big) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, AT, BT>), grid, dim3(256), 0, s, p);
+    if constexpr (!AT && !BT) {
+        if (q.rows == 64) {
+            if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
+            return launch_join(p, mode, s);
+        }
+    }
+    if (q.rows == 256) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, AT, BT>), grid, dim3(256), 0, s, p);
     else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
     launch_join(p, mode, s);
@@ -839,7 +862,7 @@ struct FwdPlan {
 static FwdPlan plan_fwd(const void* a, const void* w, void* ws, int M, int N, int K, long long lda, long long ldw) {
     FwdPlan f;
     f.a = Matrix{static_cast<const bf16*>(a), lda, M, K}, f.w = Matrix{static_cast<const bf16*>(w), ldw, N, K};
-    f.plan = plan_of(M, N, pad8(K));
+    f.plan = plan_of(M, N, pad8(K), true);
     f.few = few_rows(f.a, f.w, f.plan);
     f.slabs = nullptr, f.ja.blocks = f.jw.blocks = 0;
     Arena mem{static_cast<unsigned char*>(ws)};
@@ -908,8 +931,8 @@ static BwdPlan plan_bwd(const void* dy, const void* a, const void* w, void* ws, 
     f.parts = f.n_parts > 1 ? static_cast<float*>(mem.take((unsigned long long)f.n_parts * N * 4)) : nullptr;
     f.pair = need_da && plan_pair(M, N, K, f.pw, f.pa);
     if (!f.pair) {
-        f.pw = plan_of(N, K, M);
-        if (need_da) f.pa = plan_of(M, K, pad8(N));
+        f.pw = plan_of(N, K, M, false);
+        if (need_da) f.pa = plan_of(M, K, pad8(N), false);
     }
     const unsigned long long sw = slab_bytes(f.pw, N, K), sa = need_da ? slab_bytes(f.pa, M, K) : 0ull;
     f.slabs_w = static_cast<float*>(mem.take(sw));
