@@ -1,10 +1,12 @@
 // Distillation from a teacher's top logits: the teacher's half (the k largest logits of a row with the row's logsumexp)
 // and the student's half (loss and gradient in one pass over the student's logits).
 //
-// Both work on one row per workgroup.  The row is held in registers, VPT 16-byte vectors per thread, so the logits are
-// read from memory once: at the rates of this part (a few FLOP per byte) the kernels are bound by that read and by the
-// store of the gradient.  Rows wider than the registers of a workgroup are read a second time (VPT = 0).  All arithmetic
-// is fp32; the only rounding to fewer bits is the store of the gradient in the logits' own type.
+// Both work on one row per workgroup.  distill_kernel holds the row in registers, VPT 16-byte vectors per thread, and the
+// second half of a wide one in LDS (VL vectors per thread), so the logits are read from memory once: at a few operations per
+// byte it is bound by that read and by the store of the gradient.  Rows wider than both, or not made of whole vectors, are
+// read a second time (VPT = 0).  Measured: 4096 x 131072 bf16 with both terms at T = 2 in 512 us, 4.2 TB/s read and written
+// where a copy reaches 4.9; 509 x 49999 fp32 in 47 us, 4.3 TB/s; 1536 x 1000 bf16 in 7 us, bound by the latency of its
+// reductions.  All arithmetic is fp32; the only rounding to fewer bits is the store of the gradient in the logits' own type.
 #include "common.h"
 
 #define DS_BF16 0
@@ -633,6 +635,8 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
 // in registers, and again whenever twice as much has been read; the rest of the row streams past it: the row is read once.
 // Rows on which the bound is too low (many equal values, sorted rows) or that hold a NaN or +inf are cut to exactly k
 // candidates by bisecting the value and, among equals, the class: exact, some 50 more passes over the row.
+// Measured: 2048 x 131072 bf16, k = 64, in 124 us, 4.3 TB/s; 1536 x 1000, k = 10, in 6.5 us; 3 x 50001 fp16, k = 100, in 16 us,
+// most of it the sort of some hundred candidates.
 // ------------------------------------------------------------------------------------------
 struct TopParams {
     const void* logits;

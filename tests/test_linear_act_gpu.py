@@ -323,3 +323,30 @@ def test_head_captured_recorded_and_on_another_stream(hip, device):
         torch.cuda.synchronize()
         program.replay()
         assert all(torch.equal(s, t) for s, t in zip(everything(recorded), want))
+
+
+def test_two_streams_at_once(hip, device):
+    """Workspaces belong to a call: layers whose partial sums and copies live in them, on two streams at a time."""
+    jobs = []
+    for seed, (M, N, K) in enumerate([(333, 777, 1021), (100, 96, 4000)]):
+        gen = torch.Generator().manual_seed(seed)
+        a, w = oracle.rows((M, K), gen, device=device), oracle.rows((N, K), gen, scale=K ** -0.5, device=device)
+        jobs.append((a, w, oracle.rows((M, N), gen, device=device)))
+
+    def layer(a, w, dy):
+        y, z = hip.linear_act_fwd(a, w, act="silu", save=True)
+        return (y, z) + hip.linear_act_bwd(a, w, dy, z, "silu")
+
+    want = [layer(*job) for job in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(layer(*jobs[n]))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for out in got[n]:
+            assert all(torch.equal(x, y) for x, y in zip(out, want[n]))
