@@ -759,6 +759,7 @@ static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da)
 static bool aligned16(const void* p) { return ((unsigned long long)p & 15) == 0; }
 static int pad8(int n) { return (n + 7) / 8 * 8; }
 static int pad64(int n) { return (n + 63) / 64 * 64; }
+static bool widths(int N, int K) { return N > 0 && K > 0 && N <= LIN_MAX_LD - 64 && K <= LIN_MAX_LD - 64; }   // (padded: still an operand)
 
 // An operand of the tile kernel: rows start at 16-byte boundaries and hold a multiple of 8 columns (zeros behind the last
 // one; a descriptor that ended inside a 4-byte word would return that word's valid half as zero too).
@@ -881,14 +882,14 @@ static FwdPlan plan_fwd(const void* a, const void* w, void* ws, int M, int N, in
 
 // bytes of workspace that pdt_linear_fwd needs for these operands
 PDT_API long long pdt_linear_fwd_workspace(const void* a, const void* w, int M, int N, int K, long long lda, long long ldw) {
-    if (M < 1 || N < 1 || K < 1) return 0;
+    if (M < 1 || !widths(N, K)) return 0;
     return (long long)plan_fwd(a, w, nullptr, M, N, K, lda, ldw).bytes;
 }
 
 // Status -1: sizes, -3: a workspace is needed (nothing was launched).  y and z: rows of ldo = N rounded up to 64 columns.
 PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const void* res, void* y, void* z, void* ws, int M, int N,
                            int K, long long lda, long long ldw, long long ldr, int ldo, int act, hipStream_t s) {
-    if (M < 0 || N < 1 || K < 1 || ldo != pad64(N) || act < 0 || act > LIN_SILU) return -1;
+    if (M < 0 || !widths(N, K) || ldo != pad64(N) || act < 0 || act > LIN_SILU) return -1;
     if (M == 0) return 0;
     const FwdPlan f = plan_fwd(a, w, ws, M, N, K, lda, ldw);
     if (f.bytes > 0 && !ws) return -3;
@@ -949,7 +950,7 @@ static BwdPlan plan_bwd(const void* dy, const void* a, const void* w, void* ws, 
 
 PDT_API long long pdt_linear_bwd_workspace(const void* dy, const void* a, const void* w, int M, int N, int K, long long lddy,
                                            long long lda, long long ldw, int act, int need_da) {
-    if (M < 1 || N < 1 || K < 1) return 0;
+    if (M < 1 || !widths(N, K)) return 0;
     return (long long)plan_bwd(dy, a, w, nullptr, M, N, K, lddy, lda, ldw, act, need_da).bytes;
 }
 
@@ -958,7 +959,7 @@ PDT_API long long pdt_linear_bwd_workspace(const void* dy, const void* a, const 
 PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const void* w, void* da, void* dw, void* dbias, void* ws,
                            int M, int N, int K, long long lddy, long long ldz, long long lda, long long ldw, long long lddw, int act,
                            int add_w, int add_b, hipStream_t s) {
-    if (M < 1 || N < 1 || K < 1 || lddw < K || lddw > 0x7fffffffll || act < 0 || act > LIN_SILU || (act != LIN_NONE && !z)) return -1;
+    if (M < 1 || !widths(N, K) || lddw < K || lddw > 0x7fffffffll || act < 0 || act > LIN_SILU || (act != LIN_NONE && !z)) return -1;
     const BwdPlan f = plan_bwd(dy, a, w, ws, M, N, K, lddy, lda, ldw, act, da != nullptr);
     if (f.pw.blocks() + (da ? f.pa.blocks() : 0) + N > 0x7fffffffll) return -1;
     if (f.bytes > 0 && !ws) return -3;

@@ -537,6 +537,7 @@ def ce_metrics(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------------------- linear with activation and residual
 LINEAR_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+MAX_WIDTH = 2 ** 22 - 64                # of a layer: 256 rows of an operand stay below 2 GiB of 32-bit offsets
 
 
 def _check_rows(what: str, name: str, t: torch.Tensor, shape) -> None:
@@ -560,6 +561,8 @@ def _check_product(what: str, a: torch.Tensor, w: torch.Tensor, act: str):
         raise ValueError(f"{what}: act must be one of {sorted(LINEAR_ACTS)}, got {act!r}")
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: a [M, K] and w [N, K] with K, N >= 1, got {tuple(a.shape)}, {tuple(w.shape)}")
+    if max(a.shape[1], w.shape[0]) > MAX_WIDTH or a.shape[0] > 2 ** 31 - 65:
+        raise ValueError(f"{what}: K and N are at most {MAX_WIDTH}, M fits 31 bits, got {tuple(a.shape)}, {tuple(w.shape)}")
     _check_rows(what, "a", a, a.shape)
     _check_rows(what, "w", w, w.shape)
     return a.shape[0], w.shape[0], a.shape[1]
@@ -616,7 +619,8 @@ def _act_slope(z: torch.Tensor, act: str) -> torch.Tensor:
 def linear_act_fwd(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
                    residual: Optional[torch.Tensor] = None, save: bool = False):
     """``(y, z)``: ``z = a w^T + bias``, ``y = act(z) + residual``, each rounded once from fp32; ``a[M, K]``, ``w[N, K]``,
-    ``residual[M, N]`` in the compute dtype with unit column stride and any row stride, ``bias[N]`` fp32.
+    ``residual[M, N]`` in the compute dtype with unit column stride and any row stride, ``bias[N]`` fp32; K and N up to
+    ``MAX_WIDTH``.
 
     ``act``: none, relu, gelu (the exact one) or silu.  ``z`` is returned with ``save`` (what :func:`linear_act_bwd` needs where
     there is an activation) and is None without it or with act none.  On the GPU ``y`` and ``z`` are views of rows padded to a

@@ -103,3 +103,15 @@ def test_refusals():
     bwd(ValueError, dw=torch.zeros(1, 5).expand(4, 5))
     bwd(ValueError, dbias=torch.zeros(3))
     bwd(TypeError, dbias=torch.zeros(4).double())
+
+
+def test_widths_beyond_32_bit_offsets_are_refused():
+    wide, one = torch.zeros(1, ref.MAX_WIDTH + 1), torch.zeros(1, 1)
+    with pytest.raises(ValueError):
+        ref.linear_act_fwd(wide, wide)
+    with pytest.raises(ValueError):
+        ref.linear_act_fwd(one, wide.t().contiguous())
+    with pytest.raises(ValueError):
+        ref.linear_act_bwd(wide, wide, one)
+    y, _ = ref.linear_act_fwd(wide[:, 1:], wide[:, 1:])
+    assert y.shape == (1, 1)

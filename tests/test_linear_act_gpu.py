@@ -350,3 +350,44 @@ def test_two_streams_at_once(hip, device):
     for n in range(2):
         for out in got[n]:
             assert all(torch.equal(x, y) for x, y in zip(out, want[n]))
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_the_largest_widths(hip, device, act):
+    """K, then N, of MAX_WIDTH: 32-bit offsets of a tile's rows end just below their limit; one more is refused."""
+    from pytorch_distributed_training_amd.ops.ref import MAX_WIDTH
+    gen = torch.Generator().manual_seed(11)
+    for M, N, K in ((70, 130, MAX_WIDTH - 3), (130, MAX_WIDTH, 8)):
+        a, w = oracle.rows((M, 16), gen, device=device), oracle.rows((N if K == 8 else 16, 16), gen, device=device)
+        a, w = (a.repeat(1, K // 16 + 1)[:, :K], w.repeat(9, K // 16 + 1)[:N, :K]) if K > 16 else (a[:, :K], w[:, :K])
+        y, z = hip.linear_act_fwd(a, w, act=act, save=True)
+        dy = y.clone()
+        da, dw, db = hip.linear_act_bwd(a, w, dy, z, act)
+        rows = slice(N - 130, N)                               # the last columns of y, or all of them
+        if K > 16:
+            turns, rest = divmod(K, 16)                        # the operands repeat every 16 columns
+            want = turns * (a[:, :16].double() @ w[:, :16].double().t()) + a[:, :rest].double() @ w[:, :rest].double().t()
+            size = (turns + 1) * (a[:, :16].double().abs() @ w[:, :16].double().abs().t())
+        else:
+            want, size = a.double() @ w[rows].double().t(), a.double().abs() @ w[rows].double().abs().t()
+        bound = (K / 32 + 32) * 2.0 ** -23 * size
+        within(z[:, rows] if z is not None else y[:, rows], want, bound * 1.01 + oracle.HALF * want.abs())
+        # gradients: of the last columns alone, from dz as the formula has it
+        g = dy.double()[:, rows] * (oracle.slope(z.double()[:, rows], act) if act != "none" else 1.0)
+        off = g.abs() * oracle.HALF * 1.01 + dy.double()[:, rows].abs() * 3e-6
+        at = a[:, -16:].double()
+        want = g.t() @ at
+        bound = off.t() @ at.abs() + (M / 32 + 32) * 2.0 ** -23 * (g.abs().t() @ at.abs())
+        within(dw[rows, -16:] if K > 16 else dw[rows], want, bound * 1.01 + oracle.HALF * (want.abs() + bound))
+        if K > 16:
+            wt = w[:, -16:].double()
+            want = g @ wt
+            bound = off @ wt.abs() + (N / 32 + 32) * 2.0 ** -23 * (g.abs() @ wt.abs())
+            within(da[:, -16:], want, bound * 1.01 + oracle.HALF * (want.abs() + bound))
+        del a, w, y, z, dy, da, dw, db
+    wide = torch.zeros(1, MAX_WIDTH + 1, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError):
+        hip.linear_act_fwd(wide, wide)
+    with pytest.raises(ValueError):
+        hip.linear_act_bwd(wide, wide, wide[:, :1])
+    assert hip._real.pdt_linear_fwd(*[None] * 7, 0, 4, MAX_WIDTH + 1, MAX_WIDTH + 1, MAX_WIDTH + 1, 0, 64, 0, None) == -1
