@@ -735,13 +735,13 @@ static Plan plan_of(long long M, long long N, long long K, bool thin) {
     return q;
 }
 
-// Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then: where neither takes the large
+// Whether dw (N x K over M) and da (M x K over N) go in one launch, and how they are cut then: unless both take the large
 // tiles.  Two workgroups on a CU take 0.75 us a step where the chip is not full, and 0.43 us per tile and CU where it is.
-// One launch / two, with dbias: 1536 x 1000 x 2048 28.4 / 44.0 us, 64 x 4096 x 4096 30.9 / 37.1, 1024 x 4096 x 4096 83.7 / 94.7,
-// 300 x 16384 x 4096 147 / 163; where one takes large tiles 2048 x 4096 x 4096 142 / 144, where both do 4096 x 4096 x 4096 279 / 242.
+// One launch / two, with dbias: 1536 x 1000 x 2048 28.0 / 44.0 us, 64 x 4096 x 4096 30.2 / 37.1, 1024 x 4096 x 4096 77.5 / 94.7;
+// where one would take large tiles 1500 x 16384 x 4096 423 / 453, 2048 x 4096 x 4096 136 / 138; both: 4096 x 4096 x 4096 261 / 231.
 static bool plan_pair(long long M, long long N, long long K, Plan& dw, Plan& da) {
     dw = plan_of(N, K, M, false), da = plan_of(M, K, N, false);
-    if (dw.rows == 256 || da.rows == 256) return false;
+    if (dw.rows == 256 && da.rows == 256) return false;
     const long long tw = (long long)cdiv(N, 128) * cdiv(K, 128), ta = (long long)cdiv(M, 128) * cdiv(K, 128);
     const int nw = cdiv(M, LIN_BK), na = cdiv(N, LIN_BK);
     long long best = -1;
@@ -821,20 +821,20 @@ static void launch_join(const GemmParams& p, int mode, hipStream_t s) {
     e.mode = mode;
     hipLaunchKernelGGL(linear_join_kernel, dim3(cdiv((long long)((e.n_pad + 7) / 8) * e.M, 256)), dim3(256), 0, s, e, p.splits);
 }
-template <bool AT, bool BT>
+template <bool T>
 static void launch_gemm(const Plan& q, const GemmParams& p, int mode, hipStream_t s) {
     const dim3 grid((unsigned)q.blocks());
-    // 128 x 128 tiles: two workgroups of 80 KB on a CU where there are that many, else one with a deeper ring
-    if constexpr (!AT && !BT) {
+    // 128 columns: two workgroups of 80 KB on a CU where there are that many, else one with a deeper ring
+    if constexpr (!T) {
         if (q.rows == 64) {
-            if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
-            else hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
+            if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 9, T, T>), grid, dim3(256), 0, s, p);
+            else hipLaunchKernelGGL((linear_gemm_kernel<64, 128, 5, T, T>), grid, dim3(256), 0, s, p);
             return launch_join(p, mode, s);
         }
     }
-    if (q.rows == 256) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, AT, BT>), grid, dim3(256), 0, s, p);
-    else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 9, AT, BT>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 5, AT, BT>), grid, dim3(256), 0, s, p);
+    if (q.rows == 256) hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, T, T>), grid, dim3(256), 0, s, p);
+    else if (grid.x <= LIN_CUS) hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 9, T, T>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((linear_gemm_kernel<128, 128, 5, T, T>), grid, dim3(256), 0, s, p);
     launch_join(p, mode, s);
 }
 
@@ -909,7 +909,7 @@ PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const
     }
     if (f.plan.blocks() > 0x7fffffffll) return -1;
     launch_pack(f.ja, f.jw, s);
-    launch_gemm<false, false>(f.plan, gemm_params(f.plan, f.a, f.w, pad8(K), e, f.slabs), OUT_BF16, s);
+    launch_gemm<false>(f.plan, gemm_params(f.plan, f.a, f.w, pad8(K), e, f.slabs), OUT_BF16, s);
     return pdt_launch_status();
 }
 
@@ -940,14 +940,9 @@ static BwdPlan plan_bwd(const void* dy, const void* a, const void* w, void* ws, 
     f.n_parts = cdiv(M, 32) < cap ? cdiv(M, 32) : (cap > 0 ? cap : 1);
     f.parts = f.n_parts > 1 ? static_cast<float*>(mem.take((unsigned long long)f.n_parts * N * 4)) : nullptr;
     f.pair = need_da && plan_pair(M, N, K, f.pw, f.pa);
-    if (!f.pair) {
-        f.pw = plan_of(N, K, M, false);
-        if (need_da) f.pa = plan_of(M, K, pad8(N), false);
-    }
-    const unsigned long long sw = slab_bytes(f.pw, N, K), sa = need_da ? slab_bytes(f.pa, M, K) : 0ull;
-    f.slabs_w = static_cast<float*>(mem.take(sw));
-    f.slabs_a = static_cast<float*>(f.pair ? mem.take(sa) : f.slabs_w);
-    if (!f.pair && sa > sw) mem.take(sa - sw);                 // (one product after the other: the same place)
+    if (!need_da) f.pw = plan_of(N, K, M, false);
+    f.slabs_w = static_cast<float*>(mem.take(slab_bytes(f.pw, N, K)));
+    f.slabs_a = static_cast<float*>(mem.take(f.pair ? slab_bytes(f.pa, M, K) : 0ull));
     f.bytes = mem.used;
     return f;
 }
@@ -988,7 +983,8 @@ PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const v
         launch_join(pa, OUT_BF16, s);
         return pdt_launch_status();
     }
-    if (da) launch_gemm<false, true>(f.pa, pa, OUT_BF16, s);
-    launch_gemm<true, true>(f.pw, pw, mode, s);
+    if (da)                                                    // (alone only with the large tiles)
+        hipLaunchKernelGGL((linear_gemm_kernel<256, 256, 5, false, true>), dim3((unsigned)f.pa.blocks()), dim3(256), 0, s, pa);
+    launch_gemm<true>(f.pw, pw, mode, s);
     return pdt_launch_status();
 }

@@ -64,7 +64,7 @@ def test_few_rows_of_many_lengths(hip, device, M):
             within(y, want, bound)
 
 
-@pytest.mark.parametrize("M,N,K", [(64, 30, 4000), (2000, 40, 60), (40, 3000, 50), (700, 2100, 1900), (2200, 2304, 2100), (60, 5000, 5000)])
+@pytest.mark.parametrize("M,N,K", [(64, 30, 4000), (2000, 40, 60), (40, 3000, 50), (700, 2100, 1900), (2200, 2304, 2100), (60, 5000, 5000), (4096, 4096, 4096)])
 def test_gradients_in_one_launch_and_apart(hip, device, M, N, K):
     gen = torch.Generator().manual_seed(N)
     a, w = oracle.rows((M, K), gen, device=device), oracle.rows((N, K), gen, scale=K ** -0.5, device=device)
