@@ -622,7 +622,8 @@ def linear_act_fwd(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
     ``residual[M, N]`` in the compute dtype with unit column stride and any row stride, ``bias[N]`` fp32; K and N up to
     ``MAX_WIDTH``.
 
-    ``act``: none, relu, gelu (the exact one) or silu.  ``z`` is returned with ``save`` (what :func:`linear_act_bwd` needs where
+    ``act``: none, relu, gelu (the exact one) or silu; on the GPU gelu and silu are zero where the factor of ``z`` is below 2^-126
+    (``z`` below -13 and -87).  ``z`` is returned with ``save`` (what :func:`linear_act_bwd` needs where
     there is an activation) and is None without it or with act none.  On the GPU ``y`` and ``z`` are views of rows padded to a
     multiple of 64 columns, as :func:`linear_fwd` returns them, the padding zero."""
     check_linear_act_fwd(a, w, bias, act, residual)
