@@ -453,7 +453,9 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const bool some = m != -INFINITY || all.st != all.st;          // a row of -inf has no distribution: it counts for nothing
     const float sum_p = *slot_sum;
     const bool soft = some && !(sum_p < 0.0f);
-    const float base = finite_or_zero(a.m);
+    const bool has_label = label >= 0 && some && p.w_hard_loss != 0.0f;
+    const bool counts = __builtin_amdgcn_readfirstlane(soft || has_label);   // neither term: what the row holds reaches nothing
+    const float base = counts ? finite_or_zero(a.m) : 0.0f;
     const float inv_st = some ? 1.0f / all.st : 0.0f, inv_s1 = some ? 1.0f / all.s1 : 0.0f;
     const float p_rest = fmaxf(1.0f - sum_p, 0.0f);
     const float q_rest = rest ? a.st * exp2_fast((a.m - m) * kt) * inv_st : 0.0f;
@@ -461,12 +463,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const float mass = sum_p + (has_rest ? p_rest : 0.0f);
     float ct = 0.0f;
     if (soft) ct = rest ? (has_rest ? p.w_soft_grad * (mass * q_rest - p_rest) / a.st : 0.0f) : p.w_soft_grad * mass * inv_st;
-    const bool has_label = label >= 0 && some;
     const float wh = has_label ? p.w_hard_grad : 0.0f;
     const float c1 = has_label ? wh * inv_s1 * (rest ? exp2_fast((a.m - m) * DS_LOG2E) : 1.0f) : 0.0f;   // (an empty row: m is -inf)
     const float cs = ct + c1;                                      // T = 1: one exponential serves both
 
     auto gradient = [&](u32x4 q, int v, bool whole) {
+        if (!counts) q = u32x4{Pack<T>::FILL, Pack<T>::FILL, Pack<T>::FILL, Pack<T>::FILL};   // (a NaN times zero is none)
         float f[E], g[E];
         Pack<T>::unpack(q, f);
 #pragma unroll
@@ -521,7 +523,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
         const float P = s_p[s], d = s_z[s] - finite_or_zero(m);
         if (soft && !(P == 0.0f)) loss += P * (logf(P) - (d * p.inv_t - log_st));
         float g = soft ? p.w_soft_grad * (mass * exp2_fast(d * kt) * inv_st - P) : 0.0f;
-        g += wh * (exp2_fast(d * DS_LOG2E) * inv_s1 - (i == label ? 1.0f : 0.0f));
+        if (has_label) g += wh * (exp2_fast(d * DS_LOG2E) * inv_s1 - (i == label ? 1.0f : 0.0f));
         dst[i] = (T)g;
         label_listed |= i == label;
     }
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
                 const float g = ct * exp2_fast(d * kt) + wh * (exp2_fast((z_label - m) * DS_LOG2E) * inv_s1 - 1.0f);
                 dst[label] = (T)g;
             }
-            if (p.w_hard_loss != 0.0f) loss += p.w_hard_loss * (logf(all.s1) + (m - z_label));
+            loss += p.w_hard_loss * (logf(all.s1) + (m - z_label));
         }
         p.row_loss[row] = loss;
     }

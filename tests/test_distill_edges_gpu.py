@@ -1,0 +1,24 @@
+"""GPU tier: distill_ce in rows that count for nothing."""
+import pytest
+import torch
+
+import _distill_edges as edges
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from pytorch_distributed_training_amd.ops import hip as hip_ops
+    return hip_ops
+
+
+WIDTHS = [5, 500, 1000, 5000, 20000, 50001, 65536, 131072, 140001]       # every way in which a row is held
+
+
+@pytest.mark.parametrize("classes", WIDTHS)
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0, 4.0])
+@pytest.mark.parametrize("tail", [False, True])
+def test_what_padding_rows_hold_reaches_nothing(hip, device, classes, temperature, tail):
+    for dtype in (torch.bfloat16, torch.float32):
+        edges.check_padding_rows(hip, device, classes, dtype, temperature, tail)
