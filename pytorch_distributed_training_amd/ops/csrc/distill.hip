@@ -452,7 +452,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const float m = all.m;
     const bool some = m != -INFINITY || all.st != all.st;          // a row of -inf has no distribution: it counts for nothing
     const float sum_p = *slot_sum;
-    const bool soft = some && !(sum_p < 0.0f);
+    const bool soft = some && !(sum_p < 0.0f) && p.w_soft_loss != 0.0f;
     const bool has_label = label >= 0 && some && p.w_hard_loss != 0.0f;
     const bool counts = __builtin_amdgcn_readfirstlane(soft || has_label);   // neither term: what the row holds reaches nothing
     const float base = counts ? finite_or_zero(a.m) : 0.0f;

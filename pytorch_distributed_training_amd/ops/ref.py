@@ -735,9 +735,10 @@ def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: tor
     columns, the padding zero, as ``linear_bwd`` takes them).
 
     Left out of the mean's numerator, never of its ``B``: the hard term of a row whose label is no class, the soft term of a row
-    without slots, everything of a row whose logits are all ``-inf``.  A slot is empty if its index is no class or its value is
-    ``-inf``; slots of one class are added up.  Where the student has nothing outside the listed classes there is no rest to
-    compare.  NaN and +inf in the logits or in a slot that counts reach the loss."""
+    without slots, everything of a row whose logits are all ``-inf``, and a term whose weight is 0 (``alpha`` 0 or 1).  A slot is
+    empty if its index is no class or its value is ``-inf``; slots of one class are added up.  Where the student has nothing outside
+    the listed classes there is no rest to compare.  NaN and +inf in the logits or in a slot reach the loss through the terms that
+    count; a row without any has a gradient of zero, whatever it holds."""
     check_distill_ce(logits, labels, values, indices, temperature, alpha, lse)
     B, N = logits.shape
     l32 = logits.float()
@@ -747,7 +748,7 @@ def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: tor
     l32 = torch.where(some, l32, torch.zeros_like(l32))
     idx = indices.long()
     filled = (idx >= 0) & (idx < N) & (values != -torch.inf)
-    taught = filled.any(dim=1, keepdim=True) & some
+    taught = filled.any(dim=1, keepdim=True) & some & (alpha != 0.0)
     t = torch.where(filled, values.float() / temperature, torch.full_like(values, -torch.inf, dtype=torch.float32))
     total = lse.float()[:, None] if lse is not None else torch.logsumexp(t, dim=1, keepdim=True)
     p = torch.where(filled, torch.exp(t - total), torch.zeros_like(t))

@@ -25,3 +25,31 @@ def check_padding_rows(ops, device, classes, dtype, temperature, tail):
             weights = 0.5 * (0.4 + 0.6 * temperature)
             bound = 2 * 4 * 5 * 2.0 ** -24 * weights + torch.finfo(dtype).eps * 1.01 * want.float().abs()
             assert ((grad[:2].float() * 3 - want.float()).abs() <= bound).all()
+
+
+def check_weight_zero(ops, device, classes, tail):
+    """alpha = 0: no soft term, whatever the slots hold; alpha = 1: no hard term, whatever the label's logit is."""
+    student, labels, values, indices, lse = oracle.inputs(4, classes, 3, torch.float32, 2.0, 7, False, tail, device)
+    bare = oracle.distill(student, labels, values, indices, 2.0, 0.0, lse)
+    tolerance = oracle.loss_tolerance(bare[0], 2.0, 0.0), oracle.grad_tolerance(bare[1], torch.float32, 4, 2.0, 0.0)
+    poor = values.clone()
+    poor[1], poor[2, 0] = math.nan, math.inf
+    gone = student.clone()
+    at = indices.long()[:, 2]
+    hit = at != labels
+    assert hit.any()
+    gone[hit, at[hit]] = -math.inf                             # the student rules out a class that the teacher lists
+    for z, v in ((student, poor), (gone, values)):
+        loss, grad = ops.distill_ce(z, labels, v, indices, 2.0, 0.0, lse)
+        want, want_grad = bare if z is student else oracle.distill(z, labels, values, torch.full_like(indices, -1), 2.0, 0.0, lse)
+        assert abs(float(loss) - float(want)) <= tolerance[0], (float(loss), float(want))
+        assert ((grad.double().cpu() - want_grad).abs() <= tolerance[1].clamp_min(2e-6)).all()
+    loss, grad = ops.distill_ce(student, None, values, indices, 2.0, 0.0, lse)
+    assert float(loss) == 0.0 and not grad.any()
+    gone = student.clone()
+    labels = torch.full_like(labels, classes - 1)
+    gone[:, classes - 1] = -math.inf
+    indices = torch.where(indices == classes - 1, torch.zeros_like(indices), indices)
+    loss, grad = ops.distill_ce(gone, labels, values, indices, 2.0, 1.0, lse)
+    want, want_grad = ops.distill_ce(gone, None, values, indices, 2.0, 1.0, lse)
+    assert math.isfinite(float(loss)) and torch.equal(loss, want) and torch.equal(grad, want_grad)

@@ -1,4 +1,4 @@
-"""GPU tier: distill_ce in rows that count for nothing."""
+"""GPU tier: distill_ce in rows that count for nothing and with a term of weight zero."""
 import pytest
 import torch
 
@@ -22,3 +22,9 @@ WIDTHS = [5, 500, 1000, 5000, 20000, 50001, 65536, 131072, 140001]       # every
 def test_what_padding_rows_hold_reaches_nothing(hip, device, classes, temperature, tail):
     for dtype in (torch.bfloat16, torch.float32):
         edges.check_padding_rows(hip, device, classes, dtype, temperature, tail)
+
+
+@pytest.mark.parametrize("classes", [9, 1000, 20000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_term_of_weight_zero_is_left_out(hip, device, classes, tail):
+    edges.check_weight_zero(hip, device, classes, tail)
