@@ -146,6 +146,24 @@ __device__ __forceinline__ float wave_reduce(float v, float identity, Op op) {
 __device__ __forceinline__ float wave_total(float v) {
     return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, ROWS, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_total(double v) {
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    v += dpp_or_zero<0x143, 0xc>(v);
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)b, 63), hi = __builtin_amdgcn_readlane((int)(unsigned)(b >> 32), 63);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
 __device__ __forceinline__ float wave_top(float v) {
     return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
@@ -237,7 +255,8 @@ __device__ __forceinline__ void accumulate(Stat& s, const float (&f)[E], float k
 // Wave 0 reads the k slots while every wave's share of the row is on its way: it merges slots of one class (one bit per
 // class in LDS finds them), and the bits also take the listed classes out of the sums of the rest: q_r is a sum of its
 // own and never 1 - (a sum close to 1), relative to the rest's own maximum, so a student that is sure of the listed
-// classes does not underflow it.  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
+// classes does not underflow it.  P_r has no such sum: it is 1 minus the listed mass, in 64 bits from the slots' exponents on (in
+// fp32 a rest of 1e-5 was off by up to 5 %).  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
 // after a barrier wave 0 rewrites the listed classes and the label (k + 1 elements).
 // ------------------------------------------------------------------------------------------
 #define DS_HEAD 256                 // bytes of the waves' statistics at the head of the LDS that is not row
@@ -255,6 +274,7 @@ struct DistillParams {
     int B, N, k, ld_out;
     int label_bytes, index_bytes, value_type;
     float inv_t, w_soft_grad, w_hard_grad, w_soft_loss, w_hard_loss;
+    double inv_t64;
 };
 
 template <typename T, int THREADS, int VPT, int VL, int MODE>
@@ -264,7 +284,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     constexpr int HELD = VL * THREADS * 16;                        // the row's second part
     Stat* part = reinterpret_cast<Stat*>(lds + HELD);              // [W + 1]
-    float* slot_sum = reinterpret_cast<float*>(part + W + 1);      // sum of P, negative: the row has no slots
+    float* slot_sum = reinterpret_cast<float*>(part + W + 1);      // sum of P (negative: the row has no slots) and P_r
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x, N = p.N, k = p.k;
     const int nv = (N + E - 1) / E;
@@ -307,7 +327,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
                                                     : (long long)static_cast<const int*>(p.indices)[oi];
             float t = ld_as_float(p.values, (long long)row * p.ld_val + s * p.st_val, p.value_type);
             const int i = li >= 0 && li < N && t != -INFINITY ? (int)li : -1;
-            t = i >= 0 ? t * p.inv_t : -INFINITY;
+            if (i < 0) t = -INFINITY;
             if (i >= 0) {
                 twice |= (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31)) & 1u;
                 if (s == lane) z_first = (float)src[i];            // (used after the pass over the row: nobody waits for it)
@@ -332,18 +352,18 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
         __builtin_amdgcn_wave_barrier();
         const bool any = __ballot(tmax != -INFINITY) != 0;         // a NaN counts: it shall reach the loss
         const float top = wave_top(tmax);
-        float total = 0.0f;
+        const double base = rest ? (double)p.lse[row] : (double)top * p.inv_t64;
+        double total = 0.0;
         for (int s = lane; s < k; s += 64) {
-            const float t = s_p[s];
-            const float e = s_idx[s] < 0 ? 0.0f : expf(t - (rest ? p.lse[row] : top));
-            s_p[s] = e;
+            const double e = s_idx[s] < 0 ? 0.0 : exp((double)s_p[s] * p.inv_t64 - base);
+            s_p[s] = (float)e;
             total += e;
         }
         total = wave_total(total);
         if (!rest && any) {
-            const float inv = 1.0f / total;
+            const float inv = 1.0f / (float)total;
             for (int s = lane; s < k; s += 64) s_p[s] *= inv;
-            total = 1.0f + (total - total);                        // 1, or NaN
+            total = 1.0 + (total - total);                         // 1, or NaN
         }
         if (__ballot(twice)) {                                     // slots of one class: the first takes the sum, in slot order
             __builtin_amdgcn_wave_barrier();
@@ -364,7 +384,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
                 s_p[s] = s_q[s] == -1.0f ? 0.0f : s_q[s];
             }
         }
-        if (lane == 0) *slot_sum = any ? total : -1.0f;
+        if (lane == 0) slot_sum[0] = any ? (float)total : -1.0f, slot_sum[1] = (float)fmax(1.0 - total, 0.0);
     }
 
     Stat mine = {-INFINITY, 0.0f, 0.0f};
@@ -451,13 +471,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const Stat all = rest ? merge<MODE>(a, part[W], kt) : a;
     const float m = all.m;
     const bool some = m != -INFINITY || all.st != all.st;          // a row of -inf has no distribution: it counts for nothing
-    const float sum_p = *slot_sum;
+    const float sum_p = slot_sum[0], p_rest = slot_sum[1];
     const bool soft = some && !(sum_p < 0.0f) && p.w_soft_loss != 0.0f;
     const bool has_label = label >= 0 && some && p.w_hard_loss != 0.0f;
     const bool counts = __builtin_amdgcn_readfirstlane(soft || has_label);   // neither term: what the row holds reaches nothing
     const float base = counts ? finite_or_zero(a.m) : 0.0f;
     const float inv_st = some ? 1.0f / all.st : 0.0f, inv_s1 = some ? 1.0f / all.s1 : 0.0f;
-    const float p_rest = fmaxf(1.0f - sum_p, 0.0f);
     const float q_rest = rest ? a.st * exp2_fast((a.m - m) * kt) * inv_st : 0.0f;
     const bool has_rest = rest && a.st > 0.0f;                     // nothing outside the list: no rest to compare
     const float mass = sum_p + (has_rest ? p_rest : 0.0f);
@@ -594,11 +613,11 @@ static void launch_distill(const DistillParams& p, int mode, hipStream_t s) {
 PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* values, const void* indices, const void* lse,
                            void* dlogits, void* row_loss, void* loss, int B, int N, int k, long long ld_in, long long ld_val,
                            long long st_val, long long ld_idx, long long st_idx, int ld_out, int type, int value_type,
-                           int label_bytes, int index_bytes, float temperature, float alpha, float grad_scale,
+                           int label_bytes, int index_bytes, double temperature, float alpha, float grad_scale,
                            hipStream_t s) {
     if (B < 0 || N < 1 || N > DS_MAX_CLASSES || k < 1 || k > DS_MAX_K || ld_out < N || ld_out % 64 != 0) return -1;
     if (type < 0 || type > 2 || value_type < 0 || value_type > 2 || (label_bytes != 4 && label_bytes != 8)) return -1;
-    if ((index_bytes != 4 && index_bytes != 8) || !(temperature > 0.0f)) return -1;
+    if ((index_bytes != 4 && index_bytes != 8) || !(temperature > 0.0)) return -1;
     if (B > 0) {
         DistillParams p;
         p.logits = logits, p.labels = labels, p.values = values, p.indices = indices;
@@ -607,14 +626,15 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
         p.ld_in = ld_in, p.ld_val = ld_val, p.ld_idx = ld_idx, p.st_val = st_val, p.st_idx = st_idx;
         p.B = B, p.N = N, p.k = k, p.ld_out = ld_out;
         p.label_bytes = label_bytes, p.index_bytes = index_bytes, p.value_type = value_type;
-        p.inv_t = 1.0f / temperature;
-        p.w_soft_loss = alpha * temperature * temperature;
+        p.inv_t64 = 1.0 / temperature;
+        p.inv_t = (float)p.inv_t64;
+        p.w_soft_loss = (float)(alpha * temperature * temperature);
         p.w_hard_loss = labels ? 1.0f - alpha : 0.0f;
-        p.w_soft_grad = alpha * temperature * grad_scale / (float)B;
+        p.w_soft_grad = (float)(alpha * temperature * grad_scale / B);
         p.w_hard_grad = p.w_hard_loss * grad_scale / (float)B;
-        const int mode = p.w_hard_loss == 0.0f || temperature == 1.0f ? EXP_ONE
-                         : temperature == 2.0f                        ? EXP_SQUARE
-                         : temperature == 4.0f                        ? EXP_FOURTH
+        const int mode = p.w_hard_loss == 0.0f || temperature == 1.0 ? EXP_ONE
+                         : temperature == 2.0                         ? EXP_SQUARE
+                         : temperature == 4.0                         ? EXP_FOURTH
                                                                       : EXP_TWO;
         if (type == DS_BF16) launch_distill<bf16>(p, mode, s);
         else if (type == DS_FP16) launch_distill<f16>(p, mode, s);

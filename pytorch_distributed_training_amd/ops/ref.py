@@ -749,9 +749,11 @@ def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: tor
     idx = indices.long()
     filled = (idx >= 0) & (idx < N) & (values != -torch.inf)
     taught = filled.any(dim=1, keepdim=True) & some & (alpha != 0.0)
-    t = torch.where(filled, values.float() / temperature, torch.full_like(values, -torch.inf, dtype=torch.float32))
-    total = lse.float()[:, None] if lse is not None else torch.logsumexp(t, dim=1, keepdim=True)
-    p = torch.where(filled, torch.exp(t - total), torch.zeros_like(t))
+    # the teacher's distribution in 64 bits: its rest is 1 minus the listed mass
+    t = torch.where(filled, values.double() / temperature, torch.full_like(values, -torch.inf, dtype=torch.float64))
+    total = lse.double()[:, None] if lse is not None else torch.logsumexp(t, dim=1, keepdim=True)
+    p64 = torch.where(filled, torch.exp(t - total), torch.zeros_like(t))
+    p = p64.float()
     at = torch.where(filled, idx, torch.full_like(idx, N))                    # one column more: a bin for empty slots
     P = torch.zeros(B, N + 1, device=l32.device).scatter_add_(1, at, p)[:, :N]
     log_q = torch.log_softmax(l32 / temperature, dim=1)
@@ -762,7 +764,7 @@ def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: tor
     if lse is not None:
         listed = torch.zeros(B, N + 1, dtype=torch.bool, device=l32.device).scatter_(1, at, True)[:, :N]
         log_r = torch.logsumexp(torch.where(listed, torch.full_like(log_q, -torch.inf), log_q), dim=1, keepdim=True)
-        p_r = (1.0 - mass).clamp_min(0.0)
+        p_r = (1.0 - p64.sum(dim=1, keepdim=True)).clamp_min(0.0).float()
         has = log_r != -torch.inf
         mass = mass + torch.where(has, p_r, torch.zeros_like(p_r))
         soft = soft + torch.where(has & (p_r > 0), p_r * (p_r.log() - log_r), torch.zeros_like(p_r))

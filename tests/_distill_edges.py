@@ -53,3 +53,31 @@ def check_weight_zero(ops, device, classes, tail):
     loss, grad = ops.distill_ce(gone, labels, values, indices, 2.0, 1.0, lse)
     want, want_grad = ops.distill_ce(gone, None, values, indices, 2.0, 1.0, lse)
     assert math.isfinite(float(loss)) and torch.equal(loss, want) and torch.equal(grad, want_grad)
+
+
+def check_small_rest(ops, device, classes, temperature):
+    """512 slots that hold all but 1e-5 of the teacher's mass, and a student as sure of them: the gradient of the classes that
+    are not listed is q_i (q_r - P_r) / q_r, with both rests some 1e-5.  Taken as 1 minus an fp32 sum, P_r is off by a percent."""
+    gen = torch.Generator().manual_seed(classes)
+    k, T = 512, temperature
+    values = (torch.randn(2, k, generator=gen) * 0.1 - math.log(k)) * T
+    indices = torch.stack([torch.randperm(classes, generator=gen)[:k] for _ in range(2)]).to(torch.int32)
+    total = torch.logsumexp(values.double() / T, 1)
+    lse = (total + 1e-5).float()
+    rest = 1.0 - torch.exp(values.double() / T - lse.double()[:, None]).sum(1)
+    assert ((rest > 5e-6) & (rest < 2e-5)).all()
+    student = torch.randn(2, classes, generator=gen) * T
+    lift = 12.0 + math.log((classes - k) / k)
+    student.scatter_(1, indices.long(), values + (lift + math.log(k)) * T)
+    loss, grad = ops.distill_ce(student.to(device), None, values.to(device), indices.to(device), T, 1.0, lse.to(device))
+    log_q = torch.log_softmax(student.double() / T, 1)
+    unlisted = torch.ones(2, classes, dtype=torch.bool).scatter_(1, indices.long(), False)
+    q = log_q.exp()
+    q_rest = torch.where(unlisted, q, torch.zeros_like(q)).sum(1, keepdim=True)
+    assert ((q_rest > 3e-6) & (q_rest < 3e-5)).all()
+    share = q / q_rest * (T / 2)
+    want = share * (q_rest - rest[:, None])
+    # fp32: exponents of up to 30 with roundings of 2^-23 in the sums and in q_i, 1e-5 of each rest; the rest itself to 2^-23
+    bound = share * 2e-5 * (q_rest + rest[:, None])
+    off = (grad.double().cpu() - want).abs()[unlisted]
+    assert (off <= bound[unlisted]).all(), (off / bound[unlisted]).max().item()

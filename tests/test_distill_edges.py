@@ -1,4 +1,4 @@
-"""CPU tier: the reference distill_ce in rows that count for nothing and with a term of weight zero."""
+"""CPU tier: the reference distill_ce in rows that count for nothing, with a term of weight zero and with a small rest."""
 import pytest
 import torch
 
@@ -15,3 +15,8 @@ def test_what_padding_rows_hold_reaches_nothing(tail, dtype):
 @pytest.mark.parametrize("tail", [False, True])
 def test_a_term_of_weight_zero_is_left_out(tail):
     edges.check_weight_zero(ref, "cpu", 30, tail)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.7, 3.0])
+def test_a_small_rest_keeps_its_digits(temperature):
+    edges.check_small_rest(ref, "cpu", 1500, temperature)

@@ -1,4 +1,4 @@
-"""GPU tier: distill_ce in rows that count for nothing and with a term of weight zero."""
+"""GPU tier: distill_ce in rows that count for nothing, with a term of weight zero and with a small rest."""
 import pytest
 import torch
 
@@ -28,3 +28,9 @@ def test_what_padding_rows_hold_reaches_nothing(hip, device, classes, temperatur
 @pytest.mark.parametrize("tail", [False, True])
 def test_a_term_of_weight_zero_is_left_out(hip, device, classes, tail):
     edges.check_weight_zero(hip, device, classes, tail)
+
+
+@pytest.mark.parametrize("classes", [1500, 9000, 70000])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 2.7, 3.0])
+def test_a_small_rest_keeps_its_digits(hip, device, classes, temperature):
+    edges.check_small_rest(hip, device, classes, temperature)
