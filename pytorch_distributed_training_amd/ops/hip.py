@@ -16,7 +16,7 @@ import torch
 
 from . import build as _build
 from .ref import MASK_NONE, MASK_RECOMPUTE, MASK_TENSOR  # noqa: F401  (re-exported)
-from .ref import LINEAR_ACTS, MAX_WIDTH, check_distill_ce, check_linear_act_bwd, check_linear_act_fwd, check_top_logits
+from .ref import LINEAR_ACTS, MAX_ROWS, MAX_WIDTH, check_distill_ce, check_linear_act_bwd, check_linear_act_fwd, check_top_logits
 
 name = "hip"
 # conv_dgrad reads the transposed copies ``wt`` only: the forward weights may be updated while backward still runs
@@ -1282,7 +1282,7 @@ def linear_act_fwd(a, w, bias=None, act: str = "none", residual=None, save: bool
     # (a single row takes the GPU 5 us: the usual case is recognised by one expression, the others by the full check)
     sa, sw = a.shape, w.shape
     if not (a.dtype is _BF16 and w.dtype is _BF16 and len(sa) == 2 and len(sw) == 2 and sa[1] == sw[1]
-            and 0 < sa[1] <= MAX_WIDTH and 0 < sw[0] <= MAX_WIDTH and sa[0] < 2 ** 31 - 64
+            and 0 < sa[1] <= MAX_WIDTH and 0 < sw[0] <= MAX_WIDTH and sa[0] <= MAX_ROWS
             and a.is_contiguous() and w.is_contiguous() and residual is None and act in LINEAR_ACTS
             and (bias is None or (bias.dtype is _F32 and bias.dim() == 1 and bias.shape[0] == sw[0] and bias.is_contiguous()))):
         check_linear_act_fwd(a, w, bias, act, residual)

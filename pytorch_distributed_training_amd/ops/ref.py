@@ -537,6 +537,7 @@ def ce_metrics(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------------------- linear with activation and residual
 LINEAR_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+MAX_ROWS = 2 ** 31 - 65                 # of any operand: row numbers are 32-bit
 MAX_WIDTH = 2 ** 22 - 64                # of a layer: 256 rows of an operand stay below 2 GiB of 32-bit offsets
 
 
@@ -561,7 +562,7 @@ def _check_product(what: str, a: torch.Tensor, w: torch.Tensor, act: str):
         raise ValueError(f"{what}: act must be one of {sorted(LINEAR_ACTS)}, got {act!r}")
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: a [M, K] and w [N, K] with K, N >= 1, got {tuple(a.shape)}, {tuple(w.shape)}")
-    if max(a.shape[1], w.shape[0]) > MAX_WIDTH or a.shape[0] > 2 ** 31 - 65:
+    if max(a.shape[1], w.shape[0]) > MAX_WIDTH or a.shape[0] > MAX_ROWS:
         raise ValueError(f"{what}: K and N are at most {MAX_WIDTH}, M fits 31 bits, got {tuple(a.shape)}, {tuple(w.shape)}")
     _check_rows(what, "a", a, a.shape)
     _check_rows(what, "w", w, w.shape)
@@ -666,8 +667,9 @@ def _check_logits(what: str, logits: torch.Tensor, temperature: float):
     shape = logits.shape
     if logits.dtype not in _LOGIT_DTYPES:
         raise TypeError(f"{what}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    if len(shape) != 2 or not 1 <= shape[1] <= MAX_CLASSES:
-        raise ValueError(f"{what}: logits must be [rows, classes] with 1 to {MAX_CLASSES} classes, got {tuple(shape)}")
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_CLASSES or shape[0] > MAX_ROWS:
+        raise ValueError(f"{what}: logits must be [rows, classes] with 1 to {MAX_CLASSES} classes and at most {MAX_ROWS} rows, "
+                         f"got {tuple(shape)}")
     if logits.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f"{what}: logits must have unit column stride")
     if not 1e-3 <= temperature <= 1e3:
