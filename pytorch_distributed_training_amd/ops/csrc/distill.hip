@@ -14,6 +14,7 @@
 #define DS_FP32 2
 #define DS_MAX_K 512
 #define DS_MAX_CLASSES 262144      // one bit per class in LDS: 32 KB
+#define DS_ROWS (1 << 21)          // rows of one launch: the threads of a grid have to fit 32 bits (1024 a row: 2^22 - 1 rows)
 
 typedef _Float16 f16;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
@@ -271,7 +272,7 @@ struct DistillParams {
     void* dlogits;
     float* row_loss;
     long long ld_in, ld_val, ld_idx, st_val, st_idx;
-    int B, N, k, ld_out;
+    int row0, N, k, ld_out;
     int label_bytes, index_bytes, value_type;
     float inv_t, w_soft_grad, w_hard_grad, w_soft_loss, w_hard_loss;
     double inv_t64;
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     Stat* part = reinterpret_cast<Stat*>(lds + HELD);              // [W + 1]
     float* slot_sum = reinterpret_cast<float*>(part + W + 1);      // sum of P (negative: the row has no slots) and P_r
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x, N = p.N, k = p.k;
+    const int row = p.row0 + blockIdx.x, N = p.N, k = p.k;
     const int nv = (N + E - 1) / E;
     unsigned* bits = reinterpret_cast<unsigned*>(lds + HELD + DS_HEAD);
     const int words = ((N + 127) / 128) * 4;                       // a whole number of 16-byte stores
@@ -568,7 +569,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
 __global__ __launch_bounds__(256) void distill_mean_kernel(const float* __restrict__ v, float* __restrict__ out, int n) {
     __shared__ double red[256];
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) s += (double)v[i];
+    for (long long i = threadIdx.x; i < n; i += 256) s += (double)v[i];
     red[threadIdx.x] = s;
     __syncthreads();
     for (int w = 128; w > 0; w >>= 1) {
@@ -579,12 +580,12 @@ __global__ __launch_bounds__(256) void distill_mean_kernel(const float* __restri
 }
 
 template <typename T, int MODE>
-static void launch_distill(const DistillParams& p, hipStream_t s) {
+static void launch_distill(const DistillParams& p, int rows, hipStream_t s) {
     constexpr int NARROW = MODE == EXP_ONE ? EXP_ONE : EXP_TWO;    // (those are bound by latency, not by exponentials)
     constexpr int E = Pack<T>::E;
     const int nv = (p.N + E - 1) / E;
     const size_t shared = DS_HEAD + (size_t)((p.N + 127) / 128) * 16 + (size_t)p.k * 16;
-    const dim3 grid(p.B);
+    const dim3 grid(rows);
     // rows that start and end at 16-byte boundaries may be copied into LDS
     const bool whole = p.N % E == 0 && p.ld_in % E == 0 && ((unsigned long long)p.logits & 15) == 0;
 #define DS_LAUNCH(TH, V, L, MD) \
@@ -602,11 +603,11 @@ static void launch_distill(const DistillParams& p, hipStream_t s) {
 }
 
 template <typename T>
-static void launch_distill(const DistillParams& p, int mode, hipStream_t s) {
-    if (mode == EXP_ONE) launch_distill<T, EXP_ONE>(p, s);
-    else if (mode == EXP_SQUARE) launch_distill<T, EXP_SQUARE>(p, s);
-    else if (mode == EXP_FOURTH) launch_distill<T, EXP_FOURTH>(p, s);
-    else launch_distill<T, EXP_TWO>(p, s);
+static void launch_distill(const DistillParams& p, int rows, int mode, hipStream_t s) {
+    if (mode == EXP_ONE) launch_distill<T, EXP_ONE>(p, rows, s);
+    else if (mode == EXP_SQUARE) launch_distill<T, EXP_SQUARE>(p, rows, s);
+    else if (mode == EXP_FOURTH) launch_distill<T, EXP_FOURTH>(p, rows, s);
+    else launch_distill<T, EXP_TWO>(p, rows, s);
 }
 
 // Status -1: an argument outside what the kernel is built for (nothing was launched).
@@ -624,7 +625,7 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
         p.lse = static_cast<const float*>(lse);
         p.dlogits = dlogits, p.row_loss = static_cast<float*>(row_loss);
         p.ld_in = ld_in, p.ld_val = ld_val, p.ld_idx = ld_idx, p.st_val = st_val, p.st_idx = st_idx;
-        p.B = B, p.N = N, p.k = k, p.ld_out = ld_out;
+        p.N = N, p.k = k, p.ld_out = ld_out;
         p.label_bytes = label_bytes, p.index_bytes = index_bytes, p.value_type = value_type;
         p.inv_t64 = 1.0 / temperature;
         p.inv_t = (float)p.inv_t64;
@@ -636,11 +637,15 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
                          : temperature == 2.0                         ? EXP_SQUARE
                          : temperature == 4.0                         ? EXP_FOURTH
                                                                       : EXP_TWO;
-        if (type == DS_BF16) launch_distill<bf16>(p, mode, s);
-        else if (type == DS_FP16) launch_distill<f16>(p, mode, s);
-        else launch_distill<float>(p, mode, s);
-        const int rc = pdt_launch_status();
-        if (rc != 0) return rc;
+        for (long long row = 0; row < B; row += DS_ROWS) {
+            const int rows = (int)(B - row < DS_ROWS ? B - row : DS_ROWS);
+            p.row0 = (int)row;
+            if (type == DS_BF16) launch_distill<bf16>(p, rows, mode, s);
+            else if (type == DS_FP16) launch_distill<f16>(p, rows, mode, s);
+            else launch_distill<float>(p, rows, mode, s);
+            const int rc = pdt_launch_status();
+            if (rc != 0) return rc;
+        }
     }
     hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(256), 0, s, (const float*)row_loss, (float*)loss, B);
     return pdt_launch_status();
@@ -666,7 +671,7 @@ struct TopParams {
     int* indices;
     float* lse;
     long long ld_in;
-    int N, k;
+    int row0, N, k;
     float inv_t;
 };
 
@@ -693,7 +698,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
     __shared__ int tally[W];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x, N = p.N, k = p.k;
+    const int row = p.row0 + blockIdx.x, N = p.N, k = p.k;
     const int nv = (N + E - 1) / E;
     const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld_in;
     const float kt = p.inv_t * DS_LOG2E;
@@ -916,9 +921,9 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
 }
 
 template <typename T>
-static void launch_top(const TopParams& p, int B, hipStream_t s) {
+static void launch_top(const TopParams& p, int B, int rows, hipStream_t s) {
     const int nv = (p.N + Pack<T>::E - 1) / Pack<T>::E;
-#define DS_LAUNCH(TH, V) hipLaunchKernelGGL((top_logits_kernel<T, TH, V>), dim3(B), dim3(TH), 0, s, p)
+#define DS_LAUNCH(TH, V) hipLaunchKernelGGL((top_logits_kernel<T, TH, V>), dim3(rows), dim3(TH), 0, s, p)
     // at least two threads per wanted logit: with fewer the bound from the thread maxima lets too many candidates pass.
     // Wide rows: small workgroups where there are rows for several on every CU (one's loads run under another's sort)
     const bool many = B >= 4 * 256;
@@ -939,8 +944,14 @@ PDT_API int pdt_top_logits(const void* logits, void* values, void* indices, void
     TopParams p;
     p.logits = logits, p.values = values, p.indices = static_cast<int*>(indices), p.lse = static_cast<float*>(lse);
     p.ld_in = ld_in, p.N = N, p.k = k, p.inv_t = 1.0f / temperature;
-    if (type == DS_BF16) launch_top<bf16>(p, B, s);
-    else if (type == DS_FP16) launch_top<f16>(p, B, s);
-    else launch_top<float>(p, B, s);
-    return pdt_launch_status();
+    for (long long row = 0; row < B; row += DS_ROWS) {
+        const int rows = (int)(B - row < DS_ROWS ? B - row : DS_ROWS);
+        p.row0 = (int)row;
+        if (type == DS_BF16) launch_top<bf16>(p, B, rows, s);
+        else if (type == DS_FP16) launch_top<f16>(p, B, rows, s);
+        else launch_top<float>(p, B, rows, s);
+        const int rc = pdt_launch_status();
+        if (rc != 0) return rc;
+    }
+    return 0;
 }
