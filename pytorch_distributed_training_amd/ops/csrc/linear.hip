@@ -669,25 +669,27 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const PackJob j0, cons
     const bool second = (int)blockIdx.x >= j0.blocks;
     const PackJob& j = second ? j1 : j0;
     const int vecs = j.ldp / 8;
-    const long long t = (long long)(blockIdx.x - (second ? j0.blocks : 0)) * 256 + threadIdx.x;
-    const long long row = t / vecs;
-    const int c = (int)(t % vecs) * 8;
-    if (row >= j.rows) return;
-    const bf16* s = j.src + row * j.ld + c;
-    u32x4 v;
-    if (c + 8 <= j.cols) v = *reinterpret_cast<const u32x4_a2*>(s);
-    else {
-        float f[8];
+    const long long first = (long long)(blockIdx.x - (second ? j0.blocks : 0)) * 256 + threadIdx.x;
+    for (long long t = first; t < (long long)j.rows * vecs; t += (long long)j.blocks * 256) {
+        const long long row = t / vecs;
+        const int c = (int)(t % vecs) * 8;
+        const bf16* s = j.src + row * j.ld + c;
+        u32x4 v;
+        if (c + 8 <= j.cols) v = *reinterpret_cast<const u32x4_a2*>(s);
+        else {
+            float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = c + e < j.cols ? (float)s[e] : 0.0f;
-        v = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+            for (int e = 0; e < 8; ++e) f[e] = c + e < j.cols ? (float)s[e] : 0.0f;
+            v = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+        }
+        *reinterpret_cast<u32x4*>(j.dst + row * j.ldp + c) = v;
     }
-    *reinterpret_cast<u32x4*>(j.dst + row * j.ldp + c) = v;
 }
 
 // ------------------------------------------------------------------------------------------ launchers
 #define LIN_MAX_LD (1 << 22)           // 256 rows of an operand stay below 2 GiB of 32-bit offsets
 #define LIN_CUS 256
+#define LIN_MAX_BLOCKS 0xffffffll                              // of 256 threads: those of a launch have to fit 32 bits
 
 // How a product is cut up.  Costs are in units of 10 ns.
 struct Plan {
@@ -797,7 +799,8 @@ static Matrix operand(const Matrix& m, Arena& ws, PackJob& job) {
     const int ldp = pad8(m.cols);
     bf16* dst = static_cast<bf16*>(ws.take((unsigned long long)m.rows * ldp * 2));
     job.src = m.p, job.dst = dst, job.ld = m.ld, job.ldp = ldp, job.rows = m.rows, job.cols = m.cols;
-    job.blocks = cdiv((long long)m.rows * (ldp / 8), 256);
+    const long long blocks = ((long long)m.rows * (ldp / 8) + 255) / 256;
+    job.blocks = (int)(blocks < LIN_MAX_BLOCKS / 4 ? blocks : LIN_MAX_BLOCKS / 4);   // (beyond, a thread copies several vectors)
     return Matrix{dst, ldp, m.rows, m.cols};
 }
 static void launch_pack(const PackJob& j0, const PackJob& j1, hipStream_t s) {
@@ -892,7 +895,7 @@ PDT_API long long pdt_linear_fwd_workspace(const void* a, const void* w, int M, 
     return (long long)plan_fwd(a, w, nullptr, M, N, K, lda, ldw).bytes;
 }
 
-// Status -1: sizes, -3: a workspace is needed (nothing was launched).  y and z: rows of ldo = N rounded up to 64 columns.
+// Status -1: sizes (or more tiles than a launch has blocks), -3: a workspace is needed (nothing was launched).  y and z: rows of ldo = N rounded up to 64 columns.
 PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const void* res, void* y, void* z, void* ws, int M, int N,
                            int K, long long lda, long long ldw, long long ldr, int ldo, int act, hipStream_t s) {
     if (M < 0 || !widths(N, K) || ldo != pad64(N) || act < 0 || act > LIN_SILU) return -1;
@@ -909,7 +912,7 @@ PDT_API int pdt_linear_fwd(const void* a, const void* w, const void* bias, const
         else hipLaunchKernelGGL((linear_rows_kernel<4, 8>), grid, dim3(512), 0, s, f.a.p, f.w.p, lda, ldw, K, e);
         return pdt_launch_status();
     }
-    if (f.plan.blocks() > 0x7fffffffll) return -1;
+    if (f.plan.blocks() > LIN_MAX_BLOCKS) return -1;
     launch_pack(f.ja, f.jw, s);
     launch_gemm<false>(f.plan, gemm_params(f.plan, f.a, f.w, pad8(K), e, f.slabs), OUT_BF16, s);
     return pdt_launch_status();
@@ -962,7 +965,7 @@ PDT_API int pdt_linear_bwd(const void* dy, const void* z, const void* a, const v
                            int add_w, int add_b, hipStream_t s) {
     if (M < 1 || !widths(N, K) || lddw < K || lddw > 0x7fffffffll || act < 0 || act > LIN_SILU || (act != LIN_NONE && !z)) return -1;
     const BwdPlan f = plan_bwd(dy, a, w, ws, M, N, K, lddy, lda, ldw, act, da != nullptr);
-    if (f.pw.blocks() + (da ? f.pa.blocks() : 0) + N > 0x7fffffffll) return -1;
+    if (f.pw.blocks() + (da ? f.pa.blocks() : 0) + cdiv(N, 64) > LIN_MAX_BLOCKS) return -1;
     if (f.bytes > 0 && !ws) return -3;
     const int cols = f.dz_out ? pad64(N) : N;
     hipLaunchKernelGGL(linear_dz_kernel, dim3(cdiv(cols, 256), f.n_parts), dim3(256), 0, s, static_cast<const bf16*>(dy),
