@@ -621,7 +621,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const bf16* __restrict__
     __shared__ float red[8][32][8];
     const int cv = threadIdx.x & 31, rr = threadIdx.x >> 5;
     const int n = (blockIdx.x * 32 + cv) * 8;
-    const int r0 = blockIdx.y * rows_per, r1 = min(r0 + rows_per, M);
+    const int r0 = blockIdx.y * rows_per, r1 = r0 + min(rows_per, M - r0);   // (r0 + rows_per may pass 2^31)
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const bool whole = n + 8 <= N;
     for (int m = r0 + rr; m < r1; m += 8) {

@@ -22,3 +22,14 @@ def test_copies_of_more_threads_than_32_bits_count(hip, device):
     for at in (0, 2 ** 24 - 100, 2 ** 25 - 100, M - 70000):
         want = (a[at:at + 70000].double() @ w.double().t()).to(torch.bfloat16)
         assert torch.equal(y[at:at + 70000], want)
+
+
+def test_the_last_rows_of_as_many_as_32_bits_number(hip, device):
+    """4096 workgroups share the rows of dbias, and the last one's end lies past 2^31."""
+    from pytorch_distributed_training_amd.ops.ref import MAX_ROWS
+    dy = torch.zeros(MAX_ROWS, 8, dtype=torch.bfloat16, device=device)
+    dy[-1000:] = 1.0
+    a = torch.ones(1, 8, dtype=torch.bfloat16, device=device).expand(MAX_ROWS, 8)
+    w = torch.ones(8, 8, dtype=torch.bfloat16, device=device)
+    _, dw, db = hip.linear_act_bwd(a, w, dy, need_da=False)
+    assert (db == 1000.0).all() and (dw == 1000.0).all()
