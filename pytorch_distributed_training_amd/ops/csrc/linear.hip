@@ -889,6 +889,16 @@ static FwdPlan plan_fwd(const void* a, const void* w, void* ws, int M, int N, in
     return f;
 }
 
+// Rows of the tiles that the cost rules give the products of a layer a [M][K], w [N][K]: forward (0), da (1), dw (2).  (Whether
+// a forward product of up to 64 rows is cut into tiles at all also depends on its operands' layout.)
+PDT_API int pdt_linear_tile_rows(int M, int N, int K, int product) {
+    if (M < 1 || !widths(N, K) || product < 0 || product > 2) return -1;
+    if (product == 0) return plan_of(M, N, pad8(K), true).rows;
+    Plan pw, pa;
+    plan_pair(M, N, K, pw, pa);
+    return product == 1 ? pa.rows : pw.rows;
+}
+
 // bytes of workspace that pdt_linear_fwd needs for these operands
 PDT_API long long pdt_linear_fwd_workspace(const void* a, const void* w, int M, int N, int K, long long lda, long long ldw) {
     if (M < 1 || !widths(N, K)) return 0;

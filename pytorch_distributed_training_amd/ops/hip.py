@@ -103,6 +103,7 @@ _sig("pdt_linear_fwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, 
 _sig("pdt_linear_bwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _vp)
 _sig("pdt_linear_fwd_workspace", _vp, _vp, _i, _i, _i, _ll, _ll)
 _sig("pdt_linear_bwd_workspace", _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i)
+_sig("pdt_linear_tile_rows", _i, _i, _i, _i)
 _real.pdt_linear_fwd_workspace.restype = _ll
 _real.pdt_linear_bwd_workspace.restype = _ll
 _sig("pdt_set_deterministic", _i)
