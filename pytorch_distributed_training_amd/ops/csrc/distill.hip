@@ -673,6 +673,7 @@ struct TopParams {
     long long ld_in;
     int row0, N, k;
     float inv_t;
+    double inv_t64;
 };
 
 // unsigned order = float order; -0 = +0, NaN on top
@@ -797,7 +798,8 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(const TopParams p) 
     if (tid == 0) {
         Stat a = part[0];
         for (int w = 1; w < W; ++w) a = merge<EXP_ONE>(a, part[w], kt);
-        p.lse[row] = finite_or_zero(a.m) * p.inv_t + logf(a.st);
+        // m / T in 64 bits: rounded with the sum, once (distill_ce subtracts it from values / T in 64 bits)
+        p.lse[row] = (float)((double)finite_or_zero(a.m) * p.inv_t64 + (double)logf(a.st));
     }
     int n = count;
     bool plain = true;                                             // no NaN, no +inf: those make the sum NaN
@@ -937,13 +939,13 @@ static void launch_top(const TopParams& p, int B, int rows, hipStream_t s) {
 
 // Status -1: an argument outside what the kernel is built for (nothing was launched).
 PDT_API int pdt_top_logits(const void* logits, void* values, void* indices, void* lse, int B, int N, int k, long long ld_in,
-                           int type, float temperature, hipStream_t s) {
-    if (B < 0 || N < 1 || k < 1 || k > DS_MAX_K || k > N || N > (1 << 24) || type < 0 || type > 2 || !(temperature > 0.0f))
+                           int type, double temperature, hipStream_t s) {
+    if (B < 0 || N < 1 || k < 1 || k > DS_MAX_K || k > N || N > (1 << 24) || type < 0 || type > 2 || !(temperature > 0.0))
         return -1;
     if (B == 0) return 0;
     TopParams p;
     p.logits = logits, p.values = values, p.indices = static_cast<int*>(indices), p.lse = static_cast<float*>(lse);
-    p.ld_in = ld_in, p.N = N, p.k = k, p.inv_t = 1.0f / temperature;
+    p.ld_in = ld_in, p.N = N, p.k = k, p.inv_t64 = 1.0 / temperature, p.inv_t = (float)p.inv_t64;
     for (long long row = 0; row < B; row += DS_ROWS) {
         const int rows = (int)(B - row < DS_ROWS ? B - row : DS_ROWS);
         p.row0 = (int)row;

@@ -98,7 +98,7 @@ _sig("pdt_bnfold_wgrad", _vp, _vp, _vp, _vp, _f, _vp, _vp, _i, _i, _vp)
 _sig("pdt_bnfold_sums", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp)
 _sig("pdt_distill_ce", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _i, _i,
      ctypes.c_double, _f, _f, _vp)
-_sig("pdt_top_logits", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _f, _vp)
+_sig("pdt_top_logits", _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, ctypes.c_double, _vp)
 _sig("pdt_linear_fwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i, _i, _vp)
 _sig("pdt_linear_bwd", _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _i, _i, _i, _vp)
 _sig("pdt_linear_fwd_workspace", _vp, _vp, _i, _i, _i, _ll, _ll)

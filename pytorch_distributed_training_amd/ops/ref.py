@@ -722,7 +722,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     idx = idx.gather(1, nan_first)[:, :k]
     values = logits.gather(1, idx)
     idx = torch.where(values == -torch.inf, torch.full_like(idx, -1), idx)
-    return values, idx.to(torch.int32), torch.logsumexp(l32 / temperature, dim=1)
+    return values, idx.to(torch.int32), torch.logsumexp(l32.double() / temperature, dim=1).float()
 
 
 def distill_ce(logits: torch.Tensor, labels: Optional[torch.Tensor], values: torch.Tensor, indices: torch.Tensor,

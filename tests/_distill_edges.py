@@ -81,3 +81,13 @@ def check_small_rest(ops, device, classes, temperature):
     bound = share * 2e-5 * (q_rest + rest[:, None])
     off = (grad.double().cpu() - want).abs()[unlisted]
     assert (off <= bound[unlisted]).all(), (off / bound[unlisted]).max().item()
+
+
+def check_lse(ops, device, classes, temperature):
+    """Large logits: logits / T rounded once, in the result (an fp32 1 / T shifts every row by up to 2^-24 of it again)."""
+    gen = torch.Generator().manual_seed(classes)
+    logits = torch.randn(40, classes, generator=gen) * 3 + torch.arange(40)[:, None] * 8.0
+    want = torch.logsumexp(logits.double() / temperature, 1)
+    _, _, lse = ops.top_logits(logits.to(device), 3, temperature)
+    # half a step of fp32; the sum of exponentials, whose weights are off by some 2e-7 of their exponents, and its logarithm: 3e-6
+    assert ((lse.double().cpu() - want).abs() <= 2.0 ** -24 * 1.01 * want.abs() + 3e-6).all()

@@ -20,3 +20,8 @@ def test_a_term_of_weight_zero_is_left_out(tail):
 @pytest.mark.parametrize("temperature", [1.0, 2.7, 3.0])
 def test_a_small_rest_keeps_its_digits(temperature):
     edges.check_small_rest(ref, "cpu", 1500, temperature)
+
+
+@pytest.mark.parametrize("temperature", [0.7, 2.7])
+def test_lse_of_large_logits(temperature):
+    edges.check_lse(ref, "cpu", 1500, temperature)

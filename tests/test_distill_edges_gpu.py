@@ -34,3 +34,9 @@ def test_a_term_of_weight_zero_is_left_out(hip, device, classes, tail):
 @pytest.mark.parametrize("temperature", [1.0, 2.0, 2.7, 3.0])
 def test_a_small_rest_keeps_its_digits(hip, device, classes, temperature):
     edges.check_small_rest(hip, device, classes, temperature)
+
+
+@pytest.mark.parametrize("classes", [300, 1500, 9000, 70000])
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 1.3, 2.7, 3.0, 7.0])
+def test_lse_of_large_logits(hip, device, classes, temperature):
+    edges.check_lse(hip, device, classes, temperature)
