@@ -476,7 +476,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const bool soft = some && !(sum_p < 0.0f) && p.w_soft_loss != 0.0f;
     const bool has_label = label >= 0 && some && p.w_hard_loss != 0.0f;
     const bool counts = __builtin_amdgcn_readfirstlane(soft || has_label);   // neither term: what the row holds reaches nothing
-    const float base = counts ? finite_or_zero(a.m) : 0.0f;
+    const float base = finite_or_zero(a.m);
     const float inv_st = some ? 1.0f / all.st : 0.0f, inv_s1 = some ? 1.0f / all.s1 : 0.0f;
     const float q_rest = rest ? a.st * exp2_fast((a.m - m) * kt) * inv_st : 0.0f;
     const bool has_rest = rest && a.st > 0.0f;                     // nothing outside the list: no rest to compare
@@ -488,7 +488,6 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
     const float cs = ct + c1;                                      // T = 1: one exponential serves both
 
     auto gradient = [&](u32x4 q, int v, bool whole) {
-        if (!counts) q = u32x4{Pack<T>::FILL, Pack<T>::FILL, Pack<T>::FILL, Pack<T>::FILL};   // (a NaN times zero is none)
         float f[E], g[E];
         Pack<T>::unpack(q, f);
 #pragma unroll
@@ -509,7 +508,9 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const DistillParams p)
                 if (e >= repeated && c + e < N) dst[c + e] = (T)g[e];
         }
     };
-    if (VPT > 0) {
+    if (!counts) {                                                 // zeros, not NaN times zero
+        for (int c = tid * E; c < p.ld_out; c += THREADS * E) *reinterpret_cast<u32x4*>(dst + c) = u32x4{0, 0, 0, 0};
+    } else if (VPT > 0) {
         const int t = anew(tid);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
