@@ -4,9 +4,10 @@
 // Both work on one row per workgroup.  distill_kernel holds the row in registers, VPT 16-byte vectors per thread, and the
 // second half of a wide one in LDS (VL vectors per thread), so the logits are read from memory once: at a few operations per
 // byte it is bound by that read and by the store of the gradient.  Rows wider than both, or not made of whole vectors, are
-// read a second time (VPT = 0).  Measured: 4096 x 131072 bf16 with both terms at T = 2 in 512 us, 4.2 TB/s read and written
-// where a copy reaches 4.9; 509 x 49999 fp32 in 47 us, 4.3 TB/s; 1536 x 1000 bf16 in 7 us, bound by the latency of its
-// reductions.  All arithmetic is fp32; the only rounding to fewer bits is the store of the gradient in the logits' own type.
+// read a second time (VPT = 0).  Measured: 4096 x 131072 bf16 with both terms at T = 2 in 515 us, 4.2 TB/s read and written
+// where a copy reaches 4.9, and at T = 3 in 602; 509 x 49999 fp32 in 47 us, 4.3 TB/s; 1536 x 1000 bf16 in 7 us, bound by the latency
+// of its reductions.  Arithmetic is fp32, the teacher's listed mass 64-bit; the only rounding to fewer bits is the store of the
+// gradient in the logits' own type.
 #include "common.h"
 
 #define DS_BF16 0
@@ -190,7 +191,7 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 
 // How exp(z - m) of the hard term follows from exp((z - m) / T) of the soft one, e.  An exponential takes four issue slots of
 // the vector unit, and with two of them per element and pass a wide row is bound by that unit, not by memory: the powers
-// measured 4096 x 131072 in 512 us instead of 612.
+// measured 4096 x 131072 in 515 us at T = 2 instead of the 602 of T = 3.
 enum { EXP_ONE = 0,       // T = 1, or no hard term: one exponential
        EXP_TWO = 1,       // any T: a second one
        EXP_SQUARE = 2,    // T = 2: e^2
@@ -663,8 +664,9 @@ PDT_API int pdt_distill_ce(const void* logits, const void* labels, const void* v
 // in registers, and again whenever twice as much has been read; the rest of the row streams past it: the row is read once.
 // Rows on which the bound is too low (many equal values, sorted rows) or that hold a NaN or +inf are cut to exactly k
 // candidates by bisecting the value and, among equals, the class: exact, some 50 more passes over the row.
-// Measured: 2048 x 131072 bf16, k = 64, in 124 us, 4.3 TB/s; 1536 x 1000, k = 10, in 6.5 us; 3 x 50001 fp16, k = 100, in 16 us,
-// most of it the sort of some hundred candidates.
+// Measured: 2048 x 131072 bf16, k = 64, in 125 us, 4.3 TB/s; 1536 x 1000, k = 10, in 6.8 us; 3 x 50001 fp16, k = 100, in 16 us of
+// latency, by the clock 17 % the first chunk and its bound, 16 % its candidates, 16 % the rest of the row, 20 % the statistics'
+// merge and 30 % the sort of 264 to 382 candidates.
 // ------------------------------------------------------------------------------------------
 struct TopParams {
     const void* logits;

@@ -9,10 +9,13 @@
 // (buffer_load ... lds, no staging registers) and differ in how fragments are read back: ds_read_b128 for the first,
 // the transposing ds_read_b64_tr_b16 for the second.  No operand is ever transposed in memory.
 //
-// Bound by the matrix cores where the tiles fill the chip: 8192 x 4096 x 16384 forward in 785 us, 1400 TFLOP/s (the library's
-// bare product: 685 us); both gradients of 4096 x 16384 x 4096 in 865 us, 1270 TFLOP/s (the library: 870).  Smaller products
-// are bound by the latency of one tile and by launches, so they get smaller tiles, a split K or one launch for both gradients,
-// whichever the measured costs at plan_of() favour; up to 64 rows, by the weights' way through memory.
+// Sizes in this file are M x N x K of the layer or, at the cost rules, of one product: rows x columns x reduction (elsewhere in the
+// repository a layer is rows x inner x outer, M x K x N).
+//
+// Bound by the matrix cores where the tiles fill the chip: 8192 x 4096 x 16384 forward with a residual in 808 us, 1360 TFLOP/s (the
+// library's bare product: 695 us); both gradients and dbias of 4096 x 16384 x 4096 in 881 us, 1250 TFLOP/s (the library's two bare
+// products: 884).  Smaller products are bound by the latency of one tile and by launches, so they get smaller tiles, a split K or
+// one launch for both gradients, whichever the measured costs at plan_of() favour; up to 64 rows, by the weights' way through memory.
 #include "common.h"
 #include <type_traits>
 
@@ -615,6 +618,10 @@ __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(const bf16* __rest
 // dz = dy * act'(z) in bf16 (rows padded with zeros to ldz columns: it is the next products' operand) and the column sums of
 // the unrounded dz, rows_per rows per block; partial sums of several row blocks are joined in order.
 // act == none: only the sums (dz == null) or also a padded copy of dy.
+// dz is rounded because the matrix cores multiply bf16: unrounded it would be two operands, a high and a low part, and twice the
+// matrix instructions of both products.  The rounding is half a step of each dz, as where a framework keeps the gradient of an
+// activation in the compute type: 4096 x 16384 x 4096 gelu is 0.0023 off in the 2-norm, 0.0017 of it the results' own rounding.
+// dy without an activation is taken as it is.  4096 x 16384 in 80 us, 5.0 TB/s.
 __global__ __launch_bounds__(256) void linear_dz_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ z,
                                                         bf16* __restrict__ dz, float* __restrict__ sums, long long ldy,
                                                         long long ldzin, int ldz, int M, int N, int act, int rows_per, int add) {
@@ -855,7 +862,8 @@ static Epilogue plain_epilogue(void* out, int mode, int M, int N, long long ldo)
 // the caches at 7 TB/s; where there is little of both, 1024 columns of K take a wave 0.9 us and 0.05 us per row of a.  Tiles
 // are bound by w's way through memory at least, and pay for copies of what is not laid out for them.  Measured, few rows / tiles:
 // 4096 x 4096 with 1 row 8.3 / 14.0 us, with 64 rows 21.4 / 15.9; 16384 x 4096 with 4 rows 26 / 38, with 32 rows 54 / 39;
-// 276 x 7928 with 4 rows 10.1 / 15.7, with 64 rows 30 / 15.7; 777 x 1021 with 16 rows 6.4 / 12.5.
+// 276 x 7928 with 4 rows 10.2 / 11.0, with 64 rows 30 / 13.2; 777 x 1021 with 16 rows 6.4 / 12.4.  Where the two are close the rule
+// is off by up to 17 %: 1000 x 2048 with 64 rows takes 11.4 and could take 9.8, 4096 x 16384 with 16 rows 40.1 and 37.3.
 static bool few_rows(const Matrix& a, const Matrix& w, const Plan& tiles) {
     if (a.rows > 64) return false;
     const long long M = a.rows, N = w.rows, K = a.cols;
