@@ -258,7 +258,7 @@ __device__ __forceinline__ void accumulate(Stat& s, const float (&f)[E], float k
 // class in LDS finds them), and the bits also take the listed classes out of the sums of the rest: q_r is a sum of its
 // own and never 1 - (a sum close to 1), relative to the rest's own maximum, so a student that is sure of the listed
 // classes does not underflow it.  P_r has no such sum: it is 1 minus the listed mass, in 64 bits from the slots' exponents on (in
-// fp32 a rest of 1e-5 was off by up to 5 %).  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
+// fp32 a rest of 1e-5 was off by up to 6 %).  The main pass then writes c_T exp((z - m) / T) + c_1 exp(z - m) for every element, and
 // after a barrier wave 0 rewrites the listed classes and the label (k + 1 elements).
 // ------------------------------------------------------------------------------------------
 #define DS_HEAD 256                 // bytes of the waves' statistics at the head of the LDS that is not row

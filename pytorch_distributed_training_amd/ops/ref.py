@@ -621,7 +621,7 @@ def linear_act_fwd(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
                    residual: Optional[torch.Tensor] = None, save: bool = False):
     """``(y, z)``: ``z = a w^T + bias``, ``y = act(z) + residual``, each rounded once from fp32; ``a[M, K]``, ``w[N, K]``,
     ``residual[M, N]`` in the compute dtype with unit column stride and any row stride, ``bias[N]`` fp32; K and N up to
-    ``MAX_WIDTH``.
+    ``MAX_WIDTH``, M up to ``MAX_ROWS``.
 
     ``act``: none, relu, gelu (the exact one) or silu; on the GPU gelu and silu are zero where the factor of ``z`` is below 2^-126
     (``z`` below -13 and -87).  ``z`` is returned with ``save`` (what :func:`linear_act_bwd` needs where
@@ -712,7 +712,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     The ``k`` largest logits of each row in falling order, ties to the lower class, a NaN before every number; a class at
     ``-inf`` is never chosen (slots left over hold value ``-inf``, class ``-1``).  ``lse`` is ``logsumexp(logits / T)`` over the
     whole row (``-inf`` for a row that is ``-inf`` throughout).  ``logits``: bf16, fp16 or fp32, unit column stride, any row
-    stride; up to ``MAX_TOP`` slots and ``MAX_CLASSES`` classes."""
+    stride; up to ``MAX_TOP`` slots, ``MAX_CLASSES`` classes and ``MAX_ROWS`` rows."""
     check_top_logits(logits, k, temperature)
     l32 = logits.float()
     order = torch.where(l32.isnan(), torch.full_like(l32, torch.inf), l32)
